@@ -1,0 +1,60 @@
+/* mineral_memory.h — C ABI of the operators of a sequence memory (gfx950): linear attention with a decay per head, group norm
+ * with an activation on channels-last data, and a linear layer with bias, activation and residual in its epilogue.
+ *
+ * Same conventions as mineral_ppo.h: device pointers, `stream` is a hipStream_t passed as void*, 0 / negative MRL_E* status with
+ * mrl_last_error(), nothing allocates or synchronises, calls that share a workspace must not overlap, and the device that owns
+ * the pointers is the current one.  Strides are in elements; the last dimension of every tensor is contiguous.  The reference
+ * has no counterpart of these operators (its towers are mineral/nets/mlp.py, its rollout scans mineral/agents/ppo/experience.py).
+ */
+#ifndef MINERAL_MEMORY_H
+#define MINERAL_MEMORY_H
+
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define MRL_F32 0
+#define MRL_BF16 1
+#define MRL_F16 2
+
+#define MRL_ATTENTION_MAX_DIM 128   /* largest dim_k and dim_v */
+
+/* Linear attention with one decay per head:
+ *     S_t = exp(log_decay[h]) * S_{t-1} + k_t v_t^T        (S_{t-1} = 0 where resets[b][t] != 0)
+ *     o_t = scale * S_t^T q_t
+ * for every batch row b and head h, with S of dim_k x dim_v in fp32.  A reset drops whatever the state held, NaN and infinity
+ * included, and no token's output depends on a later token or on an earlier episode.  log_decay <= 0 is meant; -inf keeps nothing.
+ *   q, k : [batch][steps][heads][dim_k], v : [batch][steps][heads][dim_v] of `dtype`; strides {batch, step, head}
+ *   log_decay : [heads] fp32;  resets : [batch][steps] bytes or NULL;  initial_state : [batch][heads][dim_k][dim_v] fp32 or NULL (zero) */
+typedef struct mrl_attention {
+  int64_t batch, steps;
+  int32_t heads, dim_k, dim_v, dtype;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const float* log_decay;
+  const uint8_t* resets;
+  const float* initial_state;
+  float scale;
+} mrl_attention;
+
+/* Bytes of workspace of the forward call (backward = 0) or of the backward call (backward = 1); only the sizes are read. */
+int64_t mrl_linear_attention_workspace_bytes(const mrl_attention* p, int32_t backward);
+
+/* out : [batch][steps][heads][dim_v] of dtype, contiguous; final_state : [batch][heads][dim_k][dim_v] fp32. */
+int mrl_linear_attention(const mrl_attention* p, void* out, float* final_state, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients with respect to q, k, v (contiguous, of dtype) and the initial state (fp32); a NULL output is not computed
+ * (d_initial_state comes with dv).
+ *   d_out : [batch][steps][heads][dim_v], strides like the inputs;  d_final_state : fp32 or NULL (zero). */
+int mrl_linear_attention_backward(const mrl_attention* p, const void* d_out, const int64_t* d_out_stride_host, const float* d_final_state, void* dq,
+                                  void* dk, void* dv, float* d_initial_state, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One token per batch row (p->steps == 1, the step strides are not read, p->initial_state is not read): `state` is updated in place. */
+int mrl_linear_attention_step(const mrl_attention* p, float* state, void* out, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* MINERAL_MEMORY_H */

@@ -1,4 +1,4 @@
-"""ctypes binding of `libmineral_ppo.so` (the C ABI declared in include/mineral_ppo.h and include/mineral_replay.h).
+"""ctypes binding of `libmineral_ppo.so` (the C ABI declared in include/mineral_{ppo,replay,sac,shac,memory}.h).
 
 The library is the product: there is no Python/torch fallback.  If it has not been built (`make` at the repo
 root) importing a function from here raises immediately.
@@ -150,6 +150,23 @@ _SIGNATURES = {
 }
 EXPORTS = tuple(_SIGNATURES)
 
+
+class Attention(C.Structure):
+    """mrl_attention (include/mineral_memory.h)."""
+    _fields_ = [('batch', C.c_int64), ('steps', C.c_int64), ('heads', C.c_int32), ('dim_k', C.c_int32), ('dim_v', C.c_int32), ('dtype', C.c_int32),
+                ('q', C.c_void_p), ('k', C.c_void_p), ('v', C.c_void_p), ('q_stride', C.c_int64 * 3), ('k_stride', C.c_int64 * 3),
+                ('v_stride', C.c_int64 * 3), ('log_decay', C.c_void_p), ('resets', C.c_void_p), ('initial_state', C.c_void_p), ('scale', C.c_float)]
+
+
+# include/mineral_memory.h
+_MEMORY_SIGNATURES = {
+    'mrl_linear_attention_workspace_bytes': (C.c_int64, [C.POINTER(Attention), C.c_int32]),
+    'mrl_linear_attention': (C.c_int, [C.POINTER(Attention), _P, _P, _P, C.c_int64, _P]),
+    'mrl_linear_attention_backward': (C.c_int, [C.POINTER(Attention), _P, C.POINTER(C.c_int64), _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    'mrl_linear_attention_step': (C.c_int, [C.POINTER(Attention), _P, _P, _P]),
+}
+MEMORY_EXPORTS = tuple(_MEMORY_SIGNATURES)
+
 _lib = None
 
 
@@ -167,7 +184,7 @@ def lib():
             handle = C.CDLL(LIB_PATH)
         except OSError as e:
             raise HipLibraryError(f'cannot load {LIB_PATH}: {e}') from e
-        for name, (res, args) in _SIGNATURES.items():
+        for name, (res, args) in (*_SIGNATURES.items(), *_MEMORY_SIGNATURES.items()):
             try:
                 fn = getattr(handle, name)
             except AttributeError as e:

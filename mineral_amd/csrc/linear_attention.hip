@@ -1,0 +1,805 @@
+// Linear attention with one decay per head for gfx950: whole sequences in chunks, their gradient, and single tokens.
+//
+//   S_t = lambda S_{t-1} + k_t v_t^T (S_{t-1} dropped where token t begins an episode),   o_t = S_t^T q_t
+//
+// A chunk of C tokens that starts with the state S needs three products and one update (i, j inside the chunk, same episode):
+//   P_ij = lambda^(i-j) q_i.k_j (i >= j),   o_i = sum_j P_ij v_j + lambda^(i+1) S^T q_i,   S <- lambda^C S + sum_j lambda^(C-1-j) k_j v_j^T
+// The gradients are the same scan with the operands in other places: dq = scan(do, v; k), and, backwards in time,
+// dk = scan(v, do; q), dv = scan(k, q; do), whose state is the gradient of S (the last one's end is the initial state's gradient).
+// Backwards the decay follows a token's write instead of preceding it (`off` 0 instead of 1).  One kernel serves all four.
+//
+// Layout: one block per (batch row, head, segment of the tokens, slice of the value columns), 2 or 4 waves, each wave owning 16
+// (or 32) value columns and all rows of S in MFMA accumulators for the whole segment.  The products are arranged so that every
+// intermediate is the next product's operand where it lies: with 16x16x32 MFMAs a lane's accumulators of two stacked 16-row tiles
+// are rows {4g..4g+3, 16+4g..16+4g+3} of its column (g = lane / 16), and any order of the reduction index serves as long as both
+// operands share it, so S and P^T go from accumulators to operands without LDS; row-major operands are read from LDS as two
+// 8-byte pieces in that order, token-major ones through the transposing LDS read, whose 16-lane groups return exactly four rows of
+// a column.  Only q, k, v pass through LDS (registers hold the next chunk meanwhile).  The scores are computed by every wave:
+// matrix work is not what bounds the kernel, an exchange through LDS with its barriers would.
+//
+// Precision: everything accumulates in fp32.  16-bit inputs multiply as they are (fp16 as two exact bf16 terms where the partner
+// is an fp32 intermediate, whose range fp16 lacks); an fp32 intermediate enters a product as two bf16 terms (P, S: 2^-17 relative,
+// below the rounding of the 16-bit outputs) or three (the weighted v of the state, which stays fp32: 2^-24).  fp32 inputs use the
+// fp32 MFMA throughout.
+//
+// Masked tokens: weights are applied by selection, and a chunk that holds an infinity or NaN is walked token by token (the same
+// code with chunks of one), so that a zero weight never meets one: nothing of a later token or an earlier episode leaks.
+#include "memory_common.hip.h"
+
+using namespace mrl::mem;
+
+namespace {
+
+constexpr int MAX_ROLES = 3;
+
+struct Role {
+  const void *q, *k, *v;
+  int64_t qs[3], ks[3], vs[3];   // batch, step (negative: backwards in time), head; elements
+  void* out;
+  int64_t os[3];
+  const uint8_t* resets;         // of the first token in walking order, or null
+  int64_t rs[2];                 // batch, step
+  const float* s0;               // state on entry, element (row, col) at row * s_row + col * s_col; or null
+  float* s1;                     // state at the end, or null
+  int s_row, s_col;
+  int dq, dv;                    // reduction width (q, k), output width (v)
+  int off;                       // decays between the state on entry and the first token's reading
+  float oscale, wscale;          // factor of the outputs; factor of every k v^T
+  int vec;                       // all rows of q, k, v are whole 16-byte units on 16-byte addresses
+  int64_t ws;                    // this role's place in the workspace, floats
+};
+
+struct ScanP {
+  Role role[MAX_ROLES];
+  const float* log_decay;
+  float* ws;
+  int* flags;                    // [role][split][bh]: a reset inside that segment
+  int T, seg, n_splits, H;
+  int BH;
+};
+
+__device__ __forceinline__ double log2_decay(const float* log_decay, int h) { return (double)log_decay[h] * 1.4426950408889634; }
+// decay ** n; n <= 0 gives 1, also for a decay of zero.  The exponent is formed in 64 bits, so a long distance loses nothing.
+__device__ __forceinline__ float decay_pow(double l2, int n) {
+  if (n <= 0) return 1.0f;
+  const double x = l2 * n;
+  if (x < -1000.0) return 0.0f;
+  const double w = __builtin_rint(x);
+  return __builtin_ldexpf(__builtin_amdgcn_exp2f((float)(x - w)), (int)fmin(w, 2000.0));
+}
+
+// ---- element types ----------------------------------------------------------------------------------------------------------
+// Raw: a fragment as it comes from LDS; In: the same as operand next to an fp32 intermediate; De: an fp32 intermediate as operand of
+// an output's product; Wt: as operand of the state's.
+struct Planes1 { bf16x8 p[1]; };
+struct Planes2 { bf16x8 p[2]; };
+struct Planes3 { bf16x8 p[3]; };
+
+__device__ __forceinline__ Planes2 split2(const f32x8 x) {
+  Planes2 r;
+  u32x4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+    l[e] = pack_bf16(x[2 * e] - half_lo(h[e]), x[2 * e + 1] - half_hi(h[e]));
+  }
+  r.p[0] = __builtin_bit_cast(bf16x8, h);
+  r.p[1] = __builtin_bit_cast(bf16x8, l);
+  return r;
+}
+__device__ __forceinline__ Planes3 split3(const f32x8 x) {
+  Planes3 r;
+  u32x4 h, m, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+    const float a = x[2 * e] - half_lo(h[e]), b = x[2 * e + 1] - half_hi(h[e]);
+    m[e] = pack_bf16(a, b);
+    l[e] = pack_bf16(a - half_lo(m[e]), b - half_hi(m[e]));
+  }
+  r.p[0] = __builtin_bit_cast(bf16x8, h);
+  r.p[1] = __builtin_bit_cast(bf16x8, m);
+  r.p[2] = __builtin_bit_cast(bf16x8, l);
+  return r;
+}
+__device__ __forceinline__ f32x4 mfma_bf(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ void mma(f32x4& c, const Planes1& a, const Planes2& b) {
+  c = mfma_bf(a.p[0], b.p[1], c);
+  c = mfma_bf(a.p[0], b.p[0], c);
+}
+__device__ __forceinline__ void mma(f32x4& c, const Planes2& a, const Planes1& b) {
+  c = mfma_bf(a.p[1], b.p[0], c);
+  c = mfma_bf(a.p[0], b.p[0], c);
+}
+__device__ __forceinline__ void mma(f32x4& c, const Planes2& a, const Planes2& b) {   // the product of both low terms is below 2^-16
+  c = mfma_bf(a.p[1], b.p[0], c);
+  c = mfma_bf(a.p[0], b.p[1], c);
+  c = mfma_bf(a.p[0], b.p[0], c);
+}
+__device__ __forceinline__ void mma(f32x4& c, const Planes1& a, const Planes3& b) {
+  c = mfma_bf(a.p[0], b.p[2], c);
+  c = mfma_bf(a.p[0], b.p[1], c);
+  c = mfma_bf(a.p[0], b.p[0], c);
+}
+__device__ __forceinline__ void mma(f32x4& c, const Planes2& a, const Planes3& b) {   // without the 2^-25 of both lowest terms
+  c = mfma_bf(a.p[0], b.p[2], c);
+  c = mfma_bf(a.p[1], b.p[1], c);
+  c = mfma_bf(a.p[1], b.p[0], c);
+  c = mfma_bf(a.p[0], b.p[1], c);
+  c = mfma_bf(a.p[0], b.p[0], c);
+}
+__device__ __forceinline__ void mma(f32x4& c, const f32x8& a, const f32x8& b) {       // step e reduces over rows {4g + e} of a 16-row half
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+}
+
+template <typename T> struct El;
+template <> struct El<float> {
+  static constexpr int C = 32;
+  typedef f32x8 Raw; typedef f32x8 In; typedef f32x8 De; typedef f32x8 Wt;
+  static __device__ __forceinline__ In in(const Raw& r) { return r; }
+  static __device__ __forceinline__ De de(const f32x8& x) { return x; }
+  static __device__ __forceinline__ Wt wt(const f32x8& x) { return x; }
+  static __device__ __forceinline__ f32x8 wide(const Raw& r) { return r; }
+  static __device__ __forceinline__ void score(f32x4& c, const Raw& a, const Raw& b) { mma(c, a, b); }
+};
+template <> struct El<__bf16> {
+  static constexpr int C = 64;
+  typedef bf16x8 Raw; typedef Planes1 In; typedef Planes2 De; typedef Planes3 Wt;
+  static __device__ __forceinline__ In in(const Raw& r) { return Planes1{{r}}; }
+  static __device__ __forceinline__ De de(const f32x8& x) { return split2(x); }
+  static __device__ __forceinline__ Wt wt(const f32x8& x) { return split3(x); }
+  static __device__ __forceinline__ f32x8 wide(const Raw& r) {
+    const u32x4 w = __builtin_bit_cast(u32x4, r);
+    f32x8 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { x[2 * e] = half_lo(w[e]); x[2 * e + 1] = half_hi(w[e]); }
+    return x;
+  }
+  static __device__ __forceinline__ void score(f32x4& c, const Raw& a, const Raw& b) { c = mfma_bf(a, b, c); }
+};
+template <> struct El<_Float16> {
+  static constexpr int C = 64;
+  typedef f16x8 Raw; typedef Planes2 In; typedef Planes2 De; typedef Planes3 Wt;
+  static __device__ __forceinline__ f32x8 wide(const Raw& r) { return __builtin_convertvector(r, f32x8); }
+  static __device__ __forceinline__ In in(const Raw& r) { return split2(wide(r)); }   // 11 significant bits: the two terms are exact
+  static __device__ __forceinline__ De de(const f32x8& x) { return split2(x); }
+  static __device__ __forceinline__ Wt wt(const f32x8& x) { return split3(x); }
+  static __device__ __forceinline__ void score(f32x4& c, const Raw& a, const Raw& b) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ f32x8 join(const f32x4 a, const f32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// row `row` of a tile, reduction indices 32 s + {4g..4g+3, 16+4g..16+4g+3}; `tile` has PITCH bytes a row
+template <typename T, int PITCH>
+__device__ __forceinline__ typename El<T>::Raw row_frag(const char* tile, int row, int s, int g) {
+  const char* a = tile + row * PITCH + (32 * s + 4 * g) * (int)sizeof(T);
+  if constexpr (sizeof(T) == 4) {
+    return join(*reinterpret_cast<const f32x4*>(a), *reinterpret_cast<const f32x4*>(a + 64));
+  } else {
+    const u32x2 lo = *reinterpret_cast<const u32x2*>(a), hi = *reinterpret_cast<const u32x2*>(a + 32);
+    return __builtin_bit_cast(typename El<T>::Raw, __builtin_shufflevector(lo, hi, 0, 1, 2, 3));
+  }
+}
+// column col0 + lane % 16 of a tile, tokens 32 s + {4g.., 16+4g..}.  The whole wave takes part.
+template <typename T, int PITCH>
+__device__ __forceinline__ typename El<T>::Raw col_frag(const char* tile, int s, int col0, int lane) {
+  const int g = lane >> 4;
+  if constexpr (sizeof(T) == 4) {
+    const char* a = tile + (32 * s + 4 * g) * PITCH + (col0 + (lane & 15)) * 4;
+    f32x8 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = *reinterpret_cast<const float*>(a + e * PITCH);
+      x[4 + e] = *reinterpret_cast<const float*>(a + (16 + e) * PITCH);
+    }
+    return x;
+  } else {
+    // each lane names 8 bytes of a 4 x 16 block (row lane % 16 / 4, columns 4 (lane % 4)..); lane l gets column l of the block
+    typedef s16x4 __attribute__((address_space(3))) * lds_p;
+    const char* a = tile + (32 * s + 4 * g + ((lane >> 2) & 3)) * PITCH + (col0 + 4 * (lane & 3)) * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 16 * PITCH));
+    return __builtin_bit_cast(typename El<T>::Raw, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+
+// largest exponent pattern among the elements of a 16-byte unit, kept as a running maximum
+template <typename T> struct Peak;
+template <> struct Peak<float> {
+  unsigned m = 0;
+  __device__ __forceinline__ void see(const u32x4 w) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, w[e] & 0x7fffffffu);
+  }
+  __device__ __forceinline__ bool wild() const { return m >= 0x7f800000u; }
+};
+template <unsigned short INF> struct Peak16 {
+  u16x2 m = {0, 0};
+  __device__ __forceinline__ void see(const u32x4 w) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+  }
+  __device__ __forceinline__ bool wild() const { return m[0] >= INF || m[1] >= INF; }
+};
+template <> struct Peak<__bf16> : Peak16<0x7f80> {};
+template <> struct Peak<_Float16> : Peak16<0x7c00> {};
+
+template <typename T> __device__ __forceinline__ void store4(T* p, const f32x4 x, int valid, bool vec) {
+  if (vec) {
+    if (valid > 0) {
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(p) = x;
+      else {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<t4*>(p) = __builtin_convertvector(x, t4);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < valid) p[r] = (T)x[r];
+  }
+}
+
+// A [C][W] tile of tokens t .. t+n-1, columns c0 .. c0+W-1 (zero beyond `dim` and n): 16-byte units, unit u of a thread in its
+// registers between the load and the write to LDS.
+template <typename T, int C, int W, int NTH>
+struct Stage {
+  static constexpr int E = 16 / (int)sizeof(T), UPR = W / E, UNITS = C * UPR, U = (UNITS + NTH - 1) / NTH, PITCH = W * (int)sizeof(T) + 16;
+  u32x4 r[U];
+  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t step, int n, int c0, int dim, int vec, int tid) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + NTH * i, row = u / UPR, c = c0 + (u % UPR) * E;
+      u32x4 w = {0u, 0u, 0u, 0u};
+      if (row < n && c < dim) {                      // row < n <= C also keeps the unit inside the tile
+        const T* p = base + row * step + c;
+        if (vec) w = *reinterpret_cast<const u32x4*>(p);
+        else {
+          T x[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[e] = c + e < dim ? p[e] : (T)0.0f;
+          __builtin_memcpy(&w, x, 16);
+        }
+      }
+      r[i] = w;
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, int tid, Peak<T>& peak) const {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + NTH * i;
+      if (UNITS % NTH == 0 || u < UNITS) {
+        peak.see(r[i]);
+        *reinterpret_cast<u32x4*>(tile + (u / UPR) * PITCH + (u % UPR) * 16) = r[i];
+      }
+    }
+  }
+};
+
+// DP: both widths padded; NT: 16-column tiles of the values per wave; STATE: only the segment's own contribution to the state
+template <typename T, int DP, int NT, bool STATE>
+__global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const ScanP p) {
+  typedef El<T> X;
+  typedef typename X::Raw Raw;
+  typedef typename X::In In;
+  typedef typename X::De De;
+  constexpr int C = X::C, WAVES = DP == 32 ? 2 : 4, NTH = WAVES * 64, DVB = WAVES * NT * 16;
+  static_assert(DVB <= DP, "value slice");
+  constexpr int KT = DP / 16, KS = DP / 32, CT = C / 16, JS = C / 32;
+  typedef Stage<T, C, DP, NTH> SQ;
+  typedef Stage<T, C, DVB, NTH> SV;
+  __shared__ __attribute__((aligned(16))) char lq[STATE ? 16 : C * SQ::PITCH];
+  __shared__ __attribute__((aligned(16))) char lk[C * SQ::PITCH];
+  __shared__ __attribute__((aligned(16))) char lv[C * SV::PITCH];
+  __shared__ __attribute__((aligned(16))) float wj[C];
+  __shared__ int wild[2];
+
+  const Role& R = p.role[blockIdx.z];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int bh = blockIdx.x % p.BH, vt = blockIdx.x / p.BH, split = blockIdx.y;
+  const int b = bh / p.H, h = bh % p.H;
+  const int t0 = split * p.seg, t1 = min(p.T, t0 + p.seg);
+  const int c0 = vt * DVB, cw = c0 + wave * NT * 16;      // first value column of the block, of the wave
+  if (c0 >= R.dv) return;
+  const double l2 = log2_decay(p.log_decay, h);
+  const int off = R.off, dq = R.dq, dv = R.dv, vec = R.vec;
+  const T* qb = static_cast<const T*>(R.q) + b * R.qs[0] + h * R.qs[2];
+  const T* kb = static_cast<const T*>(R.k) + b * R.ks[0] + h * R.ks[2];
+  const T* vb = static_cast<const T*>(R.v) + b * R.vs[0] + h * R.vs[2];
+  T* ob = STATE ? nullptr : static_cast<T*>(R.out) + b * R.os[0] + h * R.os[2];
+  const uint8_t* rb = R.resets ? R.resets + b * R.rs[0] : nullptr;
+  const int64_t sz = (int64_t)dq * dv;
+
+  SQ sq, sk;
+  SV sv;
+  int rbyte = 0;
+  auto fetch = [&](int t, int n) {
+    if constexpr (!STATE) sq.load(qb + t * R.qs[1], R.qs[1], n, 0, dq, vec, tid);
+    sk.load(kb + t * R.ks[1], R.ks[1], n, 0, dq, vec, tid);
+    sv.load(vb + t * R.vs[1], R.vs[1], n, c0, dv, vec, tid);
+    rbyte = (rb && lane < n) ? rb[(t + lane) * R.rs[1]] : 0;
+  };
+  int t = t0, n = min(C, t1 - t0);
+  if (n > 0) fetch(t, n);
+
+  f32x4 S[KT][NT];
+  {
+    const float* s0 = nullptr;
+    int sr = R.s_row, sc = R.s_col;
+    if (!STATE) {
+      if (split == 0) s0 = R.s0 ? R.s0 + bh * sz : nullptr;
+      else { s0 = p.ws + R.ws + ((int64_t)(split - 1) * p.BH + bh) * sz; sr = dv; sc = 1; }
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * kt + 4 * g + r, col = cw + 16 * nt + m;
+          S[kt][nt][r] = (s0 && row < dq && col < dv) ? s0[(int64_t)row * sr + (int64_t)col * sc] : 0.0f;
+        }
+  }
+  // decay weights of a lane: reading (token 16 it + m), and the scores' lambda^(i-j): inside a diagonal tile directly, between tiles
+  // d + 1 apart as lambda^(16 d + m + 1) * lambda^(15 - (4g + r)), both exponents non-negative
+  float rd[CT], ai[CT], bj[4], dg[4];
+  if constexpr (!STATE) {
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      rd[i] = decay_pow(l2, 16 * i + m + off) * R.oscale;
+      ai[i] = decay_pow(l2, 16 * i + m + 1) * R.wscale * R.oscale;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      bj[r] = decay_pow(l2, 15 - (4 * g + r));
+      dg[r] = decay_pow(l2, m - (4 * g + r)) * R.wscale * R.oscale;
+    }
+  }
+  const float pC = decay_pow(l2, C);
+  bool plain_w = false;
+  int any_reset = 0, careful = t0, turn = 0;
+  if (tid < 2) wild[tid] = 0;
+  __syncthreads();
+
+  while (t < t1) {
+    // ---- stage the chunk
+    const uint64_t rm = __ballot(rbyte != 0);
+    const bool special = n != C || rm != 0;
+    if (special || !plain_w) {                          // weight of token j in the state after the chunk
+      if (tid < C) {
+        const uint64_t mj = (off ? (2ull << tid) : (1ull << tid)) - 1;
+        wj[tid] = (tid < n && (rm & ~mj) == 0) ? decay_pow(l2, n - off - tid) * R.wscale : 0.0f;
+      }
+      plain_w = !special;
+    }
+    Peak<T> peak;
+    if constexpr (!STATE) sq.store(lq, tid, peak);
+    sk.store(lk, tid, peak);
+    sv.store(lv, tid, peak);
+    if (peak.wild()) wild[turn] = 1;
+    __syncthreads();
+    const bool found = wild[turn] != 0;
+    if (tid == 0) wild[turn ^ 1] = 0;
+    turn ^= 1;
+    if (found && n > 1) {                               // walk these tokens one at a time
+      careful = t + n;
+      n = 1;
+      __syncthreads();
+      fetch(t, n);
+      continue;
+    }
+    const int tn = t + n, nn = tn < careful ? 1 : min(C, t1 - tn);
+    if (tn < t1) fetch(tn, nn);
+
+    // ---- the chunk's products
+    De sf[KS][NT];
+    if constexpr (!STATE) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sf[s][nt] = X::de(join(S[2 * s][nt], S[2 * s + 1][nt]));
+    }
+    In vin[JS][NT];
+    typename X::Wt vw[JS][NT];
+#pragma unroll
+    for (int s = 0; s < JS; ++s) {
+      const f32x8 w = join(*reinterpret_cast<const f32x4*>(wj + 32 * s + 4 * g), *reinterpret_cast<const f32x4*>(wj + 32 * s + 16 + 4 * g));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const Raw r = col_frag<T, SV::PITCH>(lv, s, wave * NT * 16 + 16 * nt, lane);
+        if constexpr (!STATE) vin[s][nt] = X::in(r);
+        vw[s][nt] = X::wt(X::wide(r) * w);
+      }
+    }
+    if constexpr (!STATE) {
+#pragma unroll
+      for (int it = 0; it < CT; ++it) {
+        if (16 * it >= n) break;
+        Raw qf[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = row_frag<T, SQ::PITCH>(lq, 16 * it + m, s, g);
+        f32x4 o[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const In qi = X::in(qf[s]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma(o[nt], sf[s][nt], qi);
+        }
+        const int i = 16 * it + m;
+        const uint64_t mi = (off ? (2ull << i) : (1ull << i)) - 1;
+        const bool reads = (rm & mi) == 0;               // no reset between the state on entry and token i
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[nt][r] = reads ? o[nt][r] * rd[it] : 0.0f;
+#pragma unroll
+        for (int s = 0; s < JS; ++s) {
+          if (2 * s > it) break;
+          f32x4 pt[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int jt = 2 * s + u;
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            if (jt <= it) {
+#pragma unroll
+              for (int ks = 0; ks < KS; ++ks) X::score(a, row_frag<T, SQ::PITCH>(lk, 16 * jt + m, ks, g), qf[ks]);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                if (jt == it) a[r] = m >= 4 * g + r ? a[r] * dg[r] : 0.0f;
+                else a[r] = a[r] * (ai[it - jt - 1] * bj[r]);
+              }
+              if (rm) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const int j = 16 * jt + 4 * g + r;
+                  const uint64_t mj = (off ? (2ull << j) : (1ull << j)) - 1;
+                  if (rm & mi & ~mj) a[r] = 0.0f;
+                }
+              }
+            }
+            pt[u] = a;
+          }
+          const De pf = X::de(join(pt[0], pt[1]));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma(o[nt], vin[s][nt], pf);
+        }
+        if (i < n) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int c = cw + 16 * nt + 4 * g;
+            store4<T>(ob + (int64_t)(t + i) * R.os[1] + c, o[nt], dv - c, (dv & 3) == 0);
+          }
+        }
+      }
+    }
+    // ---- the state after the chunk
+    const float dec = n == C ? pC : decay_pow(l2, n);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[kt][nt][r] = rm ? 0.0f : S[kt][nt][r] * dec;
+#pragma unroll
+    for (int s = 0; s < JS; ++s) {
+      if (32 * s >= n || (n == 1 && rm && !off)) break;   // a lone token whose write its own reset drops: zero times an infinity is none
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const In kc = X::in(col_frag<T, SQ::PITCH>(lk, s, 16 * kt, lane));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma(S[kt][nt], kc, vw[s][nt]);
+      }
+    }
+    any_reset |= rm != 0;
+    __syncthreads();                                     // every wave has read the tiles
+    t = tn;
+    n = nn;
+  }
+
+  float* s1 = nullptr;
+  int sr = R.s_row, sc = R.s_col;
+  if (STATE) { s1 = p.ws + R.ws + ((int64_t)split * p.BH + bh) * sz; sr = dv; sc = 1; }
+  else if (split == p.n_splits - 1) s1 = R.s1 ? R.s1 + bh * sz : nullptr;
+  if (s1) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * kt + 4 * g + r, col = cw + 16 * nt + m;
+          if (row < dq && col < dv) s1[(int64_t)row * sr + (int64_t)col * sc] = S[kt][nt][r];
+        }
+  }
+  if (STATE && vt == 0 && tid == 0) p.flags[((int64_t)blockIdx.z * p.n_splits + split) * p.BH + bh] = any_reset;
+}
+
+// Between the two passes over a split sequence: the segments' own contributions become the states on entry.  Slot s holds segment
+// s's contribution before and the state on entry of segment s + 1 after; every element walks the segments by itself.
+__global__ __launch_bounds__(256) void prefix_kernel(const ScanP p) {
+  const Role& R = p.role[blockIdx.z];
+  const int bh = blockIdx.y, h = bh % p.H;
+  const int64_t sz = (int64_t)R.dq * R.dv;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= sz) return;
+  const int row = (int)(e / R.dv), col = (int)(e % R.dv);
+  float E = R.s0 ? R.s0[bh * sz + (int64_t)row * R.s_row + (int64_t)col * R.s_col] : 0.0f;
+  const float dec = decay_pow(log2_decay(p.log_decay, h), p.seg);   // every segment but the last is whole
+  float* w = p.ws + R.ws + bh * sz + e;
+  const int* f = p.flags + (int64_t)blockIdx.z * p.n_splits * p.BH + bh;
+  const int64_t step = (int64_t)p.BH * sz;
+  const int last = p.n_splits - 1;
+  constexpr int AHEAD = 8;
+  for (int s = 0; s < last; s += AHEAD) {
+    float L[AHEAD];
+    int fl[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      L[a] = s + a < last ? w[(s + a) * step] : 0.0f;
+      fl[a] = s + a < last ? f[(int64_t)(s + a) * p.BH] : 0;
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      if (s + a < last) {
+        E = (fl[a] ? 0.0f : E * dec) + L[a];
+        w[(s + a) * step] = E;
+      }
+  }
+}
+
+// One token per row: S <- lambda S + k v^T in place, o = scale S^T q.  One block per (row, head); a thread owns VEC neighbouring
+// columns and every RG-th row of S.  Bound by the state's read and write.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void step_kernel(const mrl_attention a, float* __restrict__ state, T* __restrict__ out, int ncp) {
+  __shared__ float kq[2][MRL_ATTENTION_MAX_DIM];
+  __shared__ __attribute__((aligned(16))) float red[256 * VEC];
+  const int tid = threadIdx.x, bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads;
+  const int K = a.dim_k, V = a.dim_v;
+  const int c = (tid % ncp) * VEC, rg = tid / ncp, RG = 256 / ncp;
+  const bool clear = a.resets && a.resets[b] != 0;
+  const float dec = decay_pow(log2_decay(a.log_decay, h), 1);
+  if (tid < K) {
+    kq[0][tid] = (float)(static_cast<const T*>(a.k) + b * a.k_stride[0] + h * a.k_stride[2])[tid];
+    kq[1][tid] = (float)(static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2])[tid];
+  }
+  float v[VEC], o[VEC];
+  const T* vp = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    v[e] = c + e < V ? (float)vp[c + e] : 0.0f;
+    o[e] = 0.0f;
+  }
+  float* s = state + (int64_t)bh * K * V + c;
+  __syncthreads();
+  if (c < V) {
+    constexpr int UN = 4;
+    for (int r0 = rg; r0 < K; r0 += RG * UN) {
+      typedef float fv __attribute__((ext_vector_type(VEC)));
+      fv x[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int r = r0 + u * RG;
+        x[u] = (!clear && r < K) ? *reinterpret_cast<const fv*>(s + (int64_t)r * V) * dec : fv(0.0f);
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int r = r0 + u * RG;
+        if (r < K) {
+          const float kr = kq[0][r], qr = kq[1][r];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            x[u][e] = __builtin_fmaf(kr, v[e], x[u][e]);
+            o[e] = __builtin_fmaf(qr, x[u][e], o[e]);
+          }
+          *reinterpret_cast<fv*>(s + (int64_t)r * V) = x[u];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) red[rg * ncp * VEC + c + e] = o[e];
+  __syncthreads();
+  if (tid < V) {
+    float sum = 0.0f;
+    for (int r = 0; r < RG; ++r) sum += red[r * ncp * VEC + tid];
+    out[((int64_t)b * a.heads + h) * V + tid] = (T)(sum * a.scale);
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------
+struct Plan { int dp, nt, v_tiles, seg, n_splits; };
+
+int chunk_of(int dtype) { return dtype == MRL_F32 ? El<float>::C : El<__bf16>::C; }
+
+int check(const mrl_attention* p, const char* what) {
+  if (!p) MEM_FAIL(MRL_EINVAL, "%s: null description", what);
+  if (p->dtype < MRL_F32 || p->dtype > MRL_F16) MEM_FAIL(MRL_EINVAL, "%s: dtype %d (float32, bfloat16 or float16)", what, p->dtype);
+  if (p->batch < 0 || p->steps < 0 || p->heads < 1) MEM_FAIL(MRL_EINVAL, "%s: batch %lld, steps %lld, heads %d", what, (long long)p->batch, (long long)p->steps, p->heads);
+  if (p->dim_k < 1 || p->dim_k > MRL_ATTENTION_MAX_DIM || p->dim_v < 1 || p->dim_v > MRL_ATTENTION_MAX_DIM)
+    MEM_FAIL(MRL_EINVAL, "%s: dim_k %d, dim_v %d (1..%d each)", what, p->dim_k, p->dim_v, MRL_ATTENTION_MAX_DIM);
+  if (p->steps >= (int64_t(1) << 30)) MEM_FAIL(MRL_EINVAL, "%s: %lld steps", what, (long long)p->steps);
+  if (p->batch > (int64_t(1) << 30) / p->heads) MEM_FAIL(MRL_EINVAL, "%s: %lld batch rows x %d heads", what, (long long)p->batch, p->heads);
+  return MRL_OK;
+}
+
+int check_pointers(const mrl_attention* p, const char* what) {
+  if (p->batch == 0) return MRL_OK;
+  if (!p->log_decay) MEM_FAIL(MRL_EINVAL, "%s: null log_decay", what);
+  if (p->steps > 0 && (!p->q || !p->k || !p->v)) MEM_FAIL(MRL_EINVAL, "%s: null q, k or v", what);
+  return MRL_OK;
+}
+
+// How the work is cut.  Blocks per CU matter, not their number of tokens: with fewer than 512 blocks (two per CU) the tokens are
+// split into segments of at least four chunks, whose states are computed first, joined, and handed to the second pass.
+Plan plan_of(const mrl_attention* p, int roles) {
+  Plan r;
+  const int d = std::max(p->dim_k, p->dim_v);
+  r.dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
+  r.nt = r.dp == 128 ? 2 : 1;
+  r.v_tiles = 1;
+  const int C = chunk_of(p->dtype);
+  const int64_t blocks = std::max<int64_t>(1, p->batch * p->heads * r.v_tiles * roles);
+  const int64_t chunks = cdiv(p->steps, C);
+  int64_t splits = std::min<int64_t>(cdiv(512, blocks), chunks / 4);
+  if (splits < 2) splits = 1;
+  const int64_t per = std::max<int64_t>(1, cdiv(chunks, splits));
+  r.seg = (int)(per * C);
+  r.n_splits = (int)std::max<int64_t>(1, cdiv(chunks, per));
+  return r;
+}
+
+int64_t role_floats(const mrl_attention* p, const Plan& pl) {
+  return pl.n_splits > 1 ? (int64_t)(pl.n_splits - 1) * p->batch * p->heads * p->dim_k * p->dim_v : 0;
+}
+int64_t ws_bytes(const mrl_attention* p, const Plan& pl, int roles) {
+  if (pl.n_splits <= 1) return 0;
+  return role_floats(p, pl) * roles * 4 + (int64_t)roles * pl.n_splits * p->batch * p->heads * 4;
+}
+
+template <typename T, int DP, int NT> void launch(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
+  const unsigned gx = (unsigned)(a.BH * pl.v_tiles), nth = DP == 32 ? 128 : 256;
+  if (pl.n_splits > 1) {
+    hipLaunchKernelGGL((scan_kernel<T, DP, NT, true>), dim3(gx, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
+    const int64_t sz = (int64_t)a.role[0].dq * a.role[0].dv;
+    hipLaunchKernelGGL(prefix_kernel, dim3((unsigned)cdiv(sz, 256), a.BH, roles), dim3(256), 0, st, a);
+  }
+  hipLaunchKernelGGL((scan_kernel<T, DP, NT, false>), dim3(gx, pl.n_splits, roles), dim3(nth), 0, st, a);
+}
+template <typename T> void launch(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
+  if (pl.dp == 32) launch<T, 32, 1>(a, pl, roles, st);
+  else if (pl.dp == 64) launch<T, 64, 1>(a, pl, roles, st);
+  else launch<T, 128, 2>(a, pl, roles, st);
+}
+int dispatch(const mrl_attention* p, ScanP& a, const Plan& pl, int roles, void* ws, int64_t bytes, void* stream, const char* what) {
+  const int64_t need = ws_bytes(p, pl, roles);
+  if (need > 0 && (!ws || bytes < need)) MEM_FAIL(MRL_ENOSPC, "%s: workspace of %lld bytes, %lld needed", what, (long long)bytes, (long long)need);
+  if (need > 0 && ((uintptr_t)ws & 15)) MEM_FAIL(MRL_EINVAL, "%s: workspace is not aligned", what);
+  a.log_decay = p->log_decay;
+  a.T = (int)p->steps; a.seg = pl.seg; a.n_splits = pl.n_splits; a.H = p->heads;
+  a.BH = (int)(p->batch * p->heads);
+  a.ws = static_cast<float*>(ws);
+  for (int i = 0; i < roles; ++i) a.role[i].ws = role_floats(p, pl) * i;
+  a.flags = reinterpret_cast<int*>(a.ws + role_floats(p, pl) * roles);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p->dtype == MRL_F32) launch<float>(a, pl, roles, st);
+  else if (p->dtype == MRL_BF16) launch<__bf16>(a, pl, roles, st);
+  else launch<_Float16>(a, pl, roles, st);
+  MEM_CHECK_LAUNCH(what);
+  return MRL_OK;
+}
+
+struct Operand { const void* p; const int64_t* s; };
+
+// 16-byte loads: the width is a whole number of units, and so are the address and every stride that is used
+bool whole(const Operand& o, int dim, int es, const mrl_attention* p) {
+  const int e = 16 / es;
+  return dim % e == 0 && ((uintptr_t)o.p & 15) == 0 && (p->batch == 1 || o.s[0] % e == 0) && (p->steps <= 1 || o.s[1] % e == 0) && (p->heads == 1 || o.s[2] % e == 0);
+}
+
+void set_role(Role& r, const mrl_attention* p, bool back, const Operand& q, const Operand& k, const Operand& v, int dq, int dv, void* out) {
+  const int es = p->dtype == MRL_F32 ? 4 : 2;
+  const int64_t last = back ? p->steps - 1 : 0, sign = back ? -1 : 1;
+  auto put = [&](const void*& dst, int64_t* ds, const Operand& o) {
+    ds[0] = o.s[0]; ds[1] = sign * o.s[1]; ds[2] = o.s[2];
+    dst = static_cast<const char*>(o.p) + last * o.s[1] * es;
+  };
+  put(r.q, r.qs, q); put(r.k, r.ks, k); put(r.v, r.vs, v);
+  r.os[2] = dv; r.os[0] = p->steps * p->heads * (int64_t)dv; r.os[1] = sign * p->heads * (int64_t)dv;
+  r.out = out ? static_cast<char*>(out) + last * p->heads * (int64_t)dv * es : nullptr;
+  r.resets = p->resets ? p->resets + last : nullptr;
+  r.rs[0] = p->steps; r.rs[1] = sign;
+  r.dq = dq; r.dv = dv; r.off = back ? 0 : 1;
+  r.vec = whole(q, dq, es, p) && whole(k, dq, es, p) && whole(v, dv, es, p);
+  r.oscale = r.wscale = 1.0f;
+  r.s0 = nullptr; r.s1 = nullptr; r.s_row = dv; r.s_col = 1;
+}
+
+}  // namespace
+
+extern "C" int64_t mrl_linear_attention_workspace_bytes(const mrl_attention* p, int32_t backward) {
+  const int rc = check(p, "mrl_linear_attention_workspace_bytes");
+  if (rc) return rc;
+  const int roles = backward ? 3 : 1;
+  return ws_bytes(p, plan_of(p, roles), roles);
+}
+
+extern "C" int mrl_linear_attention(const mrl_attention* p, void* out, float* final_state, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "mrl_linear_attention";
+  int rc = check(p, what);
+  if (rc || (rc = check_pointers(p, what))) return rc;
+  if (p->batch == 0) return MRL_OK;
+  if (!final_state || (p->steps > 0 && !out)) MEM_FAIL(MRL_EINVAL, "%s: null output", what);
+  ScanP a;
+  Role& r = a.role[0];
+  set_role(r, p, false, {p->q, p->q_stride}, {p->k, p->k_stride}, {p->v, p->v_stride}, p->dim_k, p->dim_v, out);
+  r.oscale = p->scale;
+  r.s0 = p->initial_state;
+  r.s1 = final_state;
+  return dispatch(p, a, plan_of(p, 1), 1, workspace, workspace_bytes, stream, what);
+}
+
+extern "C" int mrl_linear_attention_backward(const mrl_attention* p, const void* d_out, const int64_t* d_out_stride_host, const float* d_final_state, void* dq,
+                                             void* dk, void* dv, float* d_initial_state, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "mrl_linear_attention_backward";
+  int rc = check(p, what);
+  if (rc || (rc = check_pointers(p, what))) return rc;
+  if (p->batch == 0) return MRL_OK;
+  if (p->steps > 0 && (!d_out || !d_out_stride_host)) MEM_FAIL(MRL_EINVAL, "%s: null d_out", what);
+  if (p->steps > 0 && d_initial_state && !dv) MEM_FAIL(MRL_EINVAL, "%s: d_initial_state comes with dv", what);
+  static const int64_t none[3] = {0, 0, 0};
+  const Operand q{p->q, p->q_stride}, k{p->k, p->k_stride}, v{p->v, p->v_stride}, d{d_out, d_out_stride_host ? d_out_stride_host : none};
+  const int K = p->dim_k, V = p->dim_v;
+  ScanP a;
+  int n = 0;
+  if (dq) {                 // reads S transposed
+    Role& r = a.role[n++];
+    set_role(r, p, false, d, v, k, V, K, dq);
+    r.oscale = p->scale;
+    r.s0 = p->initial_state;
+    r.s_row = 1; r.s_col = V;
+  }
+  // dk, dv: the state is the gradient of S (transposed for dk); scale belongs to every q do^T but not to d_final_state
+  if (dk) {
+    Role& r = a.role[n++];
+    set_role(r, p, true, v, d, q, V, K, dk);
+    r.wscale = p->scale;
+    r.s0 = d_final_state;
+    r.s_row = 1; r.s_col = V;
+  }
+  if (dv || d_initial_state) {
+    Role& r = a.role[n++];
+    set_role(r, p, true, k, q, d, K, V, dv);
+    r.wscale = p->scale;
+    r.s0 = d_final_state;
+    r.s1 = d_initial_state;
+  }
+  if (n == 0) return MRL_OK;
+  return dispatch(p, a, plan_of(p, 3), n, workspace, workspace_bytes, stream, what);
+}
+
+extern "C" int mrl_linear_attention_step(const mrl_attention* p, float* state, void* out, void* stream) {
+  const char* what = "mrl_linear_attention_step";
+  int rc = check(p, what);
+  if (rc || (rc = check_pointers(p, what))) return rc;
+  if (p->steps != 1) MEM_FAIL(MRL_EINVAL, "%s: %lld steps, one is meant", what, (long long)p->steps);
+  if (p->batch == 0) return MRL_OK;
+  if (!state || !out) MEM_FAIL(MRL_EINVAL, "%s: null state or output", what);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool vec = p->dim_v % 4 == 0 && ((uintptr_t)state & 15) == 0;
+  int ncp = 1;
+  while (ncp * (vec ? 4 : 1) < p->dim_v) ncp *= 2;
+  const dim3 grid((unsigned)(p->batch * p->heads)), block(256);
+  auto run = [&](auto tag) {
+    typedef decltype(tag) T;
+    if (vec) hipLaunchKernelGGL((step_kernel<T, 4>), grid, block, 0, st, *p, state, static_cast<T*>(out), ncp);
+    else hipLaunchKernelGGL((step_kernel<T, 1>), grid, block, 0, st, *p, state, static_cast<T*>(out), ncp);
+  };
+  if (p->dtype == MRL_F32) run(0.0f);
+  else if (p->dtype == MRL_BF16) run((__bf16)0.0f);
+  else run((_Float16)0.0f);
+  MEM_CHECK_LAUNCH(what);
+  return MRL_OK;
+}

@@ -139,3 +139,7 @@ for _name, _fn in (('rollout_write', _rollout_write), ('gae_finish', _gae_finish
     _lib.impl(_name, _fn, 'CUDA')
 
 OPS = ('workspace_bytes', 'param_count', 'rollout_write', 'gae_finish', 'welford_update_', 'normalize_clamp', 'policy_act', 'ppo_grad', 'clip_adam_step_')
+
+from . import memory_ops as _memory_ops  # noqa: E402  (linear attention, group norm, linear layer: include/mineral_memory.h)
+
+OPS += _memory_ops.OPS
