@@ -1,7 +1,7 @@
 # Builds the gfx950 shared library (C ABI) in-tree.  `make` here, on CPU: hipcc cross-compiles.
 HIPCC ?= /opt/rocm/bin/hipcc
 HIPFLAGS = --offload-arch=gfx950 -O3 -fPIC -shared -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-value
-SRC = mineral_amd/csrc/ppo_capi.hip mineral_amd/csrc/replay.hip mineral_amd/csrc/linear_attention.hip
+SRC = mineral_amd/csrc/ppo_capi.hip mineral_amd/csrc/replay.hip mineral_amd/csrc/linear_attention.hip mineral_amd/csrc/group_norm.hip mineral_amd/csrc/linear_act.hip
 HDR = mineral_amd/csrc/gemm.hip.h mineral_amd/csrc/chain.hip.h mineral_amd/csrc/wgrad_group.hip.h mineral_amd/csrc/split_bf16.hip.h mineral_amd/csrc/ln_wgrad0.hip.h mineral_amd/csrc/ln_fwd0.hip.h mineral_amd/csrc/ppo_tail.hip.h mineral_amd/csrc/sac_capi.hip.inc mineral_amd/csrc/shac_capi.hip.inc include/mineral_ppo.h include/mineral_replay.h include/mineral_sac.h include/mineral_shac.h
 MEMHDR = mineral_amd/csrc/memory_common.hip.h include/mineral_memory.h include/mineral_ppo.h
 OBJDIR = mineral_amd/csrc/build
@@ -14,7 +14,7 @@ $(LIB): $(OBJ)
 	$(HIPCC) $(HIPFLAGS) $(OBJ) -o $@
 
 $(OBJDIR)/ppo_capi.o $(OBJDIR)/replay.o: $(HDR)
-$(OBJDIR)/linear_attention.o: $(MEMHDR)
+$(OBJDIR)/linear_attention.o $(OBJDIR)/group_norm.o $(OBJDIR)/linear_act.o: $(MEMHDR)
 $(OBJDIR)/%.o: mineral_amd/csrc/%.hip Makefile
 	@mkdir -p $(OBJDIR)
 	$(HIPCC) $(filter-out -shared,$(HIPFLAGS)) -c $< -o $@

@@ -54,6 +54,53 @@ int mrl_linear_attention_backward(const mrl_attention* p, const void* d_out, con
 /* One token per batch row (p->steps == 1, the step strides are not read, p->initial_state is not read): `state` is updated in place. */
 int mrl_linear_attention_step(const mrl_attention* p, float* state, void* out, void* stream);
 
+#define MRL_ACT_NONE 0
+#define MRL_ACT_SILU 1
+#define MRL_ACT_ELU 2
+#define MRL_ACT_RELU 3
+#define MRL_ACT_TANH 4
+#define MRL_ACT_GELU 5   /* z Phi(z), Phi from erf */
+
+/* Group norm with an activation on channels-last data [batch][pixels][channels]: one mean and variance (divided by the count) for
+ * the pixels x channels/groups values of a sample's group,
+ *     y = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c]).
+ * x and y of `dtype`, contiguous; weight and bias [channels] of `param_dtype` (dtype or MRL_F32), NULL for one and zero. */
+typedef struct mrl_group_norm {
+  int64_t batch, pixels;
+  int32_t channels, groups, dtype, param_dtype, act;
+  float eps;
+} mrl_group_norm;
+
+/* Bytes of workspace of the forward call (backward = 0) or of the backward call (backward = 1). */
+int64_t mrl_group_norm_act_workspace_bytes(const mrl_group_norm* p, int32_t backward);
+
+/* mean, rstd : [batch][groups] fp32, what the backward call reads (either both or neither may be NULL). */
+int mrl_group_norm_act(const mrl_group_norm* p, const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* dx like x; d_weight, d_bias [channels] of param_dtype, both or neither NULL.  Sums are formed in one order: equal calls give equal bits. */
+int mrl_group_norm_act_backward(const mrl_group_norm* p, const void* x, const void* dy, const void* weight, const void* bias, const float* mean, const float* rstd,
+                                void* dx, void* d_weight, void* d_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Linear layer: y = act(x W^T + bias) + residual.
+ *   x : [rows][inputs], row stride x_stride; weight : [outputs][inputs]; bias : [outputs] or NULL; residual : [rows][outputs] or NULL;
+ *   y : [rows][outputs]; all of `dtype`, contiguous but for x.  16-bit operands multiply as they are and fp32 ones as three exact
+ *   bf16 terms (six products, error below an fp32 product's rounding); everything accumulates in fp32 and is rounded once. */
+typedef struct mrl_linear {
+  int64_t rows, x_stride;
+  int32_t inputs, outputs, dtype, act;
+} mrl_linear;
+
+/* z : [rows][outputs] of dtype or NULL: x W^T + bias, what the backward call reads where act is not MRL_ACT_NONE. */
+int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, void* stream);
+
+int64_t mrl_linear_act_backward_workspace_bytes(const mrl_linear* p);
+
+/* dx [rows][inputs], d_weight [outputs][inputs], d_bias [outputs], contiguous; a NULL output is not computed.  The residual's gradient
+ * is dy itself.  dz = dy act'(z) is rounded to dtype before the products; d_bias sums it unrounded. */
+int mrl_linear_act_backward(const mrl_linear* p, const void* x, const void* weight, const void* z, const void* dy, void* dx, void* d_weight, void* d_bias,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -158,12 +158,30 @@ class Attention(C.Structure):
                 ('v_stride', C.c_int64 * 3), ('log_decay', C.c_void_p), ('resets', C.c_void_p), ('initial_state', C.c_void_p), ('scale', C.c_float)]
 
 
+class GroupNorm(C.Structure):
+    """mrl_group_norm (include/mineral_memory.h)."""
+    _fields_ = [('batch', C.c_int64), ('pixels', C.c_int64), ('channels', C.c_int32), ('groups', C.c_int32), ('dtype', C.c_int32),
+                ('param_dtype', C.c_int32), ('act', C.c_int32), ('eps', C.c_float)]
+
+
+class Linear(C.Structure):
+    """mrl_linear (include/mineral_memory.h)."""
+    _fields_ = [('rows', C.c_int64), ('x_stride', C.c_int64), ('inputs', C.c_int32), ('outputs', C.c_int32), ('dtype', C.c_int32), ('act', C.c_int32)]
+
+
 # include/mineral_memory.h
+ACT_TYPES = {None: 0, 'SiLU': 1, 'ELU': 2, 'ReLU': 3, 'Tanh': 4, 'GELU': 5}
 _MEMORY_SIGNATURES = {
     'mrl_linear_attention_workspace_bytes': (C.c_int64, [C.POINTER(Attention), C.c_int32]),
     'mrl_linear_attention': (C.c_int, [C.POINTER(Attention), _P, _P, _P, C.c_int64, _P]),
     'mrl_linear_attention_backward': (C.c_int, [C.POINTER(Attention), _P, C.POINTER(C.c_int64), _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     'mrl_linear_attention_step': (C.c_int, [C.POINTER(Attention), _P, _P, _P]),
+    'mrl_group_norm_act_workspace_bytes': (C.c_int64, [C.POINTER(GroupNorm), C.c_int32]),
+    'mrl_group_norm_act': (C.c_int, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    'mrl_group_norm_act_backward': (C.c_int, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    'mrl_linear_act': (C.c_int, [C.POINTER(Linear), _P, _P, _P, _P, _P, _P, _P]),
+    'mrl_linear_act_backward_workspace_bytes': (C.c_int64, [C.POINTER(Linear)]),
+    'mrl_linear_act_backward': (C.c_int, [C.POINTER(Linear), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
 }
 MEMORY_EXPORTS = tuple(_MEMORY_SIGNATURES)
 

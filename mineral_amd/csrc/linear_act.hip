@@ -1,0 +1,532 @@
+// Linear layer with bias, activation and residual in its epilogue for gfx950, and its gradient:
+//   z = x W^T + b, y = act(z) + residual;   dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum dz
+// One tiled product D[m][n] = sum_r A(m, r) B(n, r) serves the three: an operand lies with the reduction index along its rows (x and
+// W forward, dz for dx) or with rows of the reduction index (W for dx, both for dW), and goes to LDS as it lies; fragments of the
+// first kind are 16-byte reads, of the second transposing reads.  Tiles travel HBM -> registers -> LDS one step ahead of the MFMAs.
+// The MFMAs take the operands swapped, so a lane's accumulators are four neighbouring columns of one row; the epilogue passes them
+// through LDS once and then works on rows: bias, z, activation, residual and stores in 16-byte units.
+// fp32 operands are split exactly into three bf16 terms on their way to LDS and multiply in six products, smallest first.
+// dW sums over all rows: they are split over blocks whose partial sums are added in a fixed order.
+#include "memory_common.hip.h"
+
+using namespace mrl::mem;
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+enum { LAY_K = 0, LAY_R = 1 };   // reduction index along the rows / rows of the reduction index
+
+struct MmP {
+  const void *a, *b;
+  int64_t lda, ldb;
+  int M, N;                 // rows of D (A's), columns (B's)
+  int64_t R;                // reduction length
+  int64_t r_split;          // reduction length of a split (a multiple of the step)
+  int m_tiles, n_tiles, blocks;
+  void* y;                  // [M][N]
+  float* slab;              // instead of y: [splits][M][N] fp32
+  const void *bias, *residual;
+  void* z;
+  int act;
+};
+
+// one 16-byte unit, elements beyond `left` zero; addresses need only the element's alignment
+template <typename T> __device__ __forceinline__ u32x4 load_unit(const T* p, int64_t left) {
+  constexpr int E = 16 / (int)sizeof(T);
+  u32x4 w = {0u, 0u, 0u, 0u};
+  if (left >= E) __builtin_memcpy(&w, p, 16);
+  else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e < left) {
+        if constexpr (sizeof(T) == 4) w[e] = __builtin_bit_cast(unsigned, p[e]);
+        else w[e / 2] |= (unsigned)__builtin_bit_cast(unsigned short, p[e]) << (16 * (e & 1));
+      }
+  }
+  return w;
+}
+
+template <typename T> struct Frag;
+template <> struct Frag<__bf16> {
+  static constexpr int NP = 1;
+  typedef bf16x8 F;
+  static __device__ __forceinline__ f32x16 mul(const F& a, const F& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<_Float16> {
+  static constexpr int NP = 1;
+  typedef f16x8 F;
+  static __device__ __forceinline__ f32x16 mul(const F& a, const F& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<float> {
+  static constexpr int NP = 3;
+  typedef bf16x8 F;
+  static __device__ __forceinline__ f32x16 mul(const F& a, const F& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+// One operand's tile: ROWS rows (of A or B) x BK reduction indices.
+template <typename T, int LAY, int ROWS, int BK, int NTH> struct Operand {
+  static constexpr int NP = Frag<T>::NP, E = 16 / (int)sizeof(T);
+  // LDS image: [ROWS][BK] or [BK][ROWS] 16-bit values, row pitches that spread the fragment reads over the banks
+  static constexpr int LINES = LAY == LAY_K ? ROWS : BK, WIDTH = LAY == LAY_K ? BK : ROWS;
+  static constexpr int PITCH = WIDTH * 2 + (LAY == LAY_K ? 16 : 64);
+  static constexpr int PLANE = LINES * PITCH, BYTES = PLANE * NP;
+  static constexpr int UPL = WIDTH / E, UNITS = LINES * UPL, U = (UNITS + NTH - 1) / NTH;
+  u32x4 r[U];
+  const T* p[U];          // this thread's units of the next tile
+  int64_t left[U];        // elements up to the end of the line; none where the line is outside
+
+  // row0: first row of the tile; lines beyond `rows` (LAY_K) or beyond r1 (LAY_R) read as zero
+  __device__ __forceinline__ void init(const void* base, int64_t ld, int64_t row0, int64_t rows, int64_t r0, int64_t r1, int tid) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + NTH * i, line = u / UPL, c = (u % UPL) * E;
+      if constexpr (LAY == LAY_K) {
+        p[i] = static_cast<const T*>(base) + (row0 + line) * ld + r0 + c;
+        left[i] = (u < UNITS && row0 + line < rows) ? r1 - r0 - c : 0;
+      } else {
+        p[i] = static_cast<const T*>(base) + (r0 + line) * ld + row0 + c;
+        left[i] = u < UNITS ? rows - row0 - c : 0;
+      }
+    }
+  }
+  __device__ __forceinline__ void load(int64_t ld, int64_t r0, int64_t r1, int tid) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int line = (tid + NTH * i) / UPL;
+      if constexpr (LAY == LAY_K) {
+        r[i] = load_unit(p[i], left[i]);
+        p[i] += BK;
+        left[i] -= BK;
+      } else {
+        r[i] = load_unit(p[i], r0 + line < r1 ? left[i] : 0);
+        p[i] += BK * ld;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = tid + NTH * i;
+      if (UNITS % NTH == 0 || u < UNITS) {
+        char* q = tile + (u / UPL) * PITCH + (u % UPL) * E * 2;
+        if constexpr (NP == 1) *reinterpret_cast<u32x4*>(q) = r[i];
+        else {
+          u32x2 h, m, l;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x0 = __uint_as_float(r[i][2 * e]), x1 = __uint_as_float(r[i][2 * e + 1]);
+            h[e] = pack_bf16(x0, x1);
+            const float a0 = x0 - half_lo(h[e]), a1 = x1 - half_hi(h[e]);
+            m[e] = pack_bf16(a0, a1);
+            l[e] = pack_bf16(a0 - half_lo(m[e]), a1 - half_hi(m[e]));
+          }
+          *reinterpret_cast<u32x2*>(q) = h;
+          *reinterpret_cast<u32x2*>(q + PLANE) = m;
+          *reinterpret_cast<u32x2*>(q + 2 * PLANE) = l;
+        }
+      }
+    }
+  }
+  // rows row .. row + 31 (one a lane), reduction indices 16 ks + 8 (lane / 32) + 0..7
+  static __device__ __forceinline__ typename Frag<T>::F frag(const char* tile, int plane, int row, int ks, int lane) {
+    const char* t = tile + plane * PLANE;
+    if constexpr (LAY == LAY_K) {
+      return __builtin_bit_cast(typename Frag<T>::F, *reinterpret_cast<const u32x4*>(t + (row + (lane & 31)) * PITCH + (16 * ks + 8 * (lane >> 5)) * 2));
+    } else {
+      // a 16-lane group names four lines of 16 columns, 8 bytes a lane, and every lane gets its column of them
+      typedef s16x4 __attribute__((address_space(3))) * lds_p;
+      const char* a = t + (16 * ks + 8 * (lane >> 5) + ((lane >> 2) & 3)) * PITCH + (row + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 4 * PITCH));
+      return __builtin_bit_cast(typename Frag<T>::F, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+template <typename T, int N> __device__ __forceinline__ void load_row(const T* p, int left, float (&x)[N]) {
+  if (left >= N) {
+    T v[N];
+    __builtin_memcpy(v, p, sizeof(v));
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = (float)v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = e < left ? (float)p[e] : 0.0f;
+  }
+}
+template <typename T, int N> __device__ __forceinline__ void store_row(T* p, int left, const float (&x)[N]) {
+  if (left >= N) {
+    T v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = (T)x[e];
+    __builtin_memcpy(p, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < left) p[e] = (T)x[e];
+  }
+}
+
+// WM x WN waves over the tile, WK waves over the reduction inside a step
+template <typename T, int BM, int BN, int BK, int WM, int WN, int WK, int LA, int LB, int NBUF>
+__global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
+  constexpr int NTH = WM * WN * WK * 64, TM = BM / WM / 32, TN = BN / WN / 32, KS = BK / 16 / WK, NP = Frag<T>::NP;
+  typedef Operand<T, LA, BM, BK, NTH> OA;
+  typedef Operand<T, LB, BN, BK, NTH> OB;
+  typedef typename Frag<T>::F F;
+  constexpr int STAGE = OA::BYTES + OB::BYTES, EP = BN + 4, EBYTES = WK * BM * EP * 4;
+  constexpr int LDS = NBUF * STAGE > EBYTES ? NBUF * STAGE : EBYTES;
+  __shared__ __attribute__((aligned(16))) char lds[LDS];
+  // consecutive blocks go to the 8 XCDs in turn: each XCD gets a run of neighbouring tiles, so that its L2 holds what they share
+  const int tiles = p.m_tiles * p.n_tiles;
+  const int per = (gridDim.x + 7) / 8;
+  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  const int split = id / tiles, tile = id % tiles;
+  if (id >= p.blocks) return;                            // the grid is padded to a multiple of 8
+  const int64_t m0 = (int64_t)(tile / p.n_tiles) * BM;
+  const int n0 = (tile % p.n_tiles) * BN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wk = wave % WK, wn = wave / WK % WN, wm = wave / (WK * WN);
+  const int64_t r0 = split * p.r_split, r1 = min(p.R, r0 + p.r_split);
+
+  OA oa;
+  OB ob;
+  oa.init(p.a, p.lda, m0, p.M, r0, r1, tid);
+  ob.init(p.b, p.ldb, n0, p.N, r0, r1, tid);
+  f32x16 acc[TN][TM];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.0f;
+
+  const int steps = (int)((r1 - r0 + BK - 1) / BK);
+  auto multiply = [&](const char* st) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int ks = wk * KS + k;
+      F a[NP][TM], b[NP][TN];
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) a[q][i] = OA::frag(st, q, (wm * TM + i) * 32, ks, lane);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) b[q][j] = OB::frag(st + OA::BYTES, q, (wn * TN + j) * 32, ks, lane);
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          if constexpr (NP == 3) {
+            acc[j][i] = Frag<T>::mul(b[2][j], a[0][i], acc[j][i]);
+            acc[j][i] = Frag<T>::mul(b[0][j], a[2][i], acc[j][i]);
+            acc[j][i] = Frag<T>::mul(b[1][j], a[1][i], acc[j][i]);
+            acc[j][i] = Frag<T>::mul(b[1][j], a[0][i], acc[j][i]);
+            acc[j][i] = Frag<T>::mul(b[0][j], a[1][i], acc[j][i]);
+          }
+          acc[j][i] = Frag<T>::mul(b[0][j], a[0][i], acc[j][i]);
+        }
+    }
+  };
+  if (steps > 0) {
+    oa.load(p.lda, r0, r1, tid);
+    ob.load(p.ldb, r0, r1, tid);
+  }
+  if constexpr (NBUF == 2) {
+    if (steps > 0) {
+      oa.store(lds, tid);
+      ob.store(lds + OA::BYTES, tid);
+    }
+    for (int s = 0; s < steps; ++s) {
+      if (s + 1 < steps) {
+        oa.load(p.lda, r0 + (int64_t)(s + 1) * BK, r1, tid);
+        ob.load(p.ldb, r0 + (int64_t)(s + 1) * BK, r1, tid);
+      }
+      __syncthreads();                       // stage s is written, and every wave has left the one that s + 1 goes to
+      multiply(lds + (s & 1) * STAGE);
+      if (s + 1 < steps) {
+        char* next = lds + ((s + 1) & 1) * STAGE;
+        oa.store(next, tid);
+        ob.store(next + OA::BYTES, tid);
+      }
+    }
+  } else {
+    for (int s = 0; s < steps; ++s) {
+      oa.store(lds, tid);
+      ob.store(lds + OA::BYTES, tid);
+      if (s + 1 < steps) {
+        oa.load(p.lda, r0 + (int64_t)(s + 1) * BK, r1, tid);
+        ob.load(p.ldb, r0 + (int64_t)(s + 1) * BK, r1, tid);
+      }
+      __syncthreads();
+      multiply(lds);
+      __syncthreads();
+    }
+  }
+
+  // ---- epilogue: rows of the tile from LDS
+  __syncthreads();
+  float* ep = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = wk * BM + (wm * TM + i) * 32 + (lane & 31), col = (wn * TN + j) * 32 + 8 * q + 4 * (lane >> 5);
+        *reinterpret_cast<f32x4*>(ep + row * EP + col) = f32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+      }
+  __syncthreads();
+  constexpr int UPR = BN / 8;
+  for (int u = tid; u < BM * UPR; u += NTH) {
+    const int row = u / UPR, c = (u % UPR) * 8;
+    const int64_t m = m0 + row;
+    const int left = p.N - n0 - c;
+    if (m >= p.M || left <= 0) continue;
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 s = *reinterpret_cast<const f32x4*>(ep + row * EP + c + 4 * h);
+#pragma unroll
+      for (int k = 1; k < WK; ++k) s += *reinterpret_cast<const f32x4*>(ep + (k * BM + row) * EP + c + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * h + e] = s[e];
+    }
+    const int64_t at = m * p.N + n0 + c;
+    if (p.slab) {
+      store_row<float, 8>(p.slab + (int64_t)split * p.M * p.N + at, left, v);
+      continue;
+    }
+    if (p.bias) {
+      float b[8];
+      load_row<T, 8>(static_cast<const T*>(p.bias) + n0 + c, left, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += b[e];
+    }
+    if (p.z) store_row<T, 8>(static_cast<T*>(p.z) + at, left, v);
+    act_fwd<8>(p.act, v);
+    if (p.residual) {
+      float b[8];
+      load_row<T, 8>(static_cast<const T*>(p.residual) + at, left, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += b[e];
+    }
+    store_row<T, 8>(static_cast<T*>(p.y) + at, left, v);
+  }
+}
+
+// dz = dy act'(z), and the sums of its columns over this block's rows -> part [blocks in y][N].  32 units of 8 columns x 8 rows a block.
+template <typename T>
+__global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ z, const T* __restrict__ dy, T* __restrict__ dz, float* __restrict__ part, int64_t M, int N, int act,
+                                                 int rows) {
+  __shared__ float red[8][32 * 8 + 1];
+  const int cu = threadIdx.x & 31, rl = threadIdx.x >> 5;
+  const int c = (blockIdx.x * 32 + cu) * 8, left = N - c;
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+  if (left > 0) {
+    const int64_t m1 = min(M, ((int64_t)blockIdx.y + 1) * rows);
+    for (int64_t m = (int64_t)blockIdx.y * rows + rl; m < m1; m += 8) {
+      float d[8], zz[8];
+      load_row<T, 8>(dy + m * N + c, left, d);
+      if (z) {
+        load_row<T, 8>(z + m * N + c, left, zz);
+        act_bwd<8>(act, zz, d);
+        store_row<T, 8>(dz + m * N + c, left, d);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += d[e];
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) red[rl][cu * 8 + e] = s[e];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col < N) {
+    float a = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a += red[k][threadIdx.x];
+    part[(int64_t)blockIdx.y * N + col] = a;
+  }
+}
+
+// out[c] = sum over rows of part [rows][n]: 32 columns a block, 32 threads a column
+template <typename T>
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ part, int64_t rows, int n, T* __restrict__ out) {
+  __shared__ float red[32][33];
+  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
+  float a = 0.0f;
+  if (c < n) {
+    constexpr int U = 8;
+    for (int64_t r = rl; r < rows; r += 32 * U) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = r + 32 * u < rows ? part[(r + 32 * u) * n + c] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) a += v[u];
+    }
+  }
+  red[rl][cl] = a;
+  __syncthreads();
+  if (rl == 0 && c < n) {
+    float s = 0.0f;
+    for (int k = 0; k < 32; ++k) s += red[k][cl];
+    out[c] = (T)s;
+  }
+}
+
+// dW = sum of the splits' slabs, four values a thread
+template <typename T>
+__global__ __launch_bounds__(256) void slab_sum_kernel(const float* __restrict__ slab, int splits, int64_t n, T* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int left = (int)min<int64_t>(4, n - i);
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < splits; ++k) {
+    float v[4];
+    load_row<float, 4>(slab + k * n + i, left, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += v[e];
+  }
+  store_row<T, 4>(out + i, left, s);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+int check(const mrl_linear* p, const char* what) {
+  if (!p) MEM_FAIL(MRL_EINVAL, "%s: null description", what);
+  if (p->dtype < MRL_F32 || p->dtype > MRL_F16) MEM_FAIL(MRL_EINVAL, "%s: dtype %d (float32, bfloat16 or float16)", what, p->dtype);
+  if (p->act < MRL_ACT_NONE || p->act > MRL_ACT_GELU) MEM_FAIL(MRL_EINVAL, "%s: activation %d", what, p->act);
+  if (p->rows < 0 || p->inputs < 0 || p->outputs < 0) MEM_FAIL(MRL_EINVAL, "%s: rows %lld, inputs %d, outputs %d", what, (long long)p->rows, p->inputs, p->outputs);
+  if (p->rows > (int64_t(1) << 30) || p->inputs > (1 << 24) || p->outputs > (1 << 24)) MEM_FAIL(MRL_EINVAL, "%s: sizes beyond 2^30 rows or 2^24 columns", what);
+  if (p->rows > 1 && p->x_stride < p->inputs) MEM_FAIL(MRL_EINVAL, "%s: x_stride %lld below %d inputs", what, (long long)p->x_stride, p->inputs);
+  if (cdiv(p->rows, 32) * cdiv(std::max(p->inputs, p->outputs), 32) >= (int64_t(1) << 30)) MEM_FAIL(MRL_EINVAL, "%s: too many tiles", what);
+  return MRL_OK;
+}
+
+// Tile edge: 128 where its tiles fill the card, otherwise smaller ones, whose reduction is shared by the block's waves at 32.
+int edge_of(int64_t m, int64_t n) {
+  if (cdiv(m, 128) * cdiv(n, 128) >= 256) return 128;
+  if (cdiv(m, 64) * cdiv(n, 64) >= 256) return 64;
+  return 32;
+}
+
+template <typename T, int LA, int LB> void multiply(MmP& a, int edge, int splits, hipStream_t st) {
+  a.m_tiles = (int)cdiv(a.M, edge);
+  a.n_tiles = (int)cdiv(a.N, edge);
+  a.blocks = a.m_tiles * a.n_tiles * splits;
+  const dim3 grid((unsigned)(cdiv(a.blocks, 8) * 8));
+  constexpr bool F32 = sizeof(T) == 4;
+  if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, F32 ? 32 : 64, 2, 2, 1, LA, LB, F32 ? 1 : 2>), grid, dim3(256), 0, st, a);
+  else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, F32 ? 32 : 64, 2, 2, 1, LA, LB, F32 ? 1 : 2>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, F32 ? 1 : 2>), grid, dim3(256), 0, st, a);
+}
+
+struct Plan { int edge_x, edge_w, splits; int64_t r_split; int rows, parts; int64_t dz, part, slab, total; };
+
+Plan plan_of(const mrl_linear* p) {
+  Plan r{};
+  const int64_t es = p->dtype == MRL_F32 ? 4 : 2;
+  r.edge_x = edge_of(p->rows, p->inputs);
+  // dW: 128 x 128 tiles where both widths have them; rows split so that about 512 blocks run, in whole steps of 64
+  r.edge_w = std::min(p->inputs, p->outputs) >= 96 ? 128 : std::min(p->inputs, p->outputs) >= 48 ? 64 : 32;
+  const int64_t tiles = std::max<int64_t>(1, cdiv(p->outputs, r.edge_w) * cdiv(p->inputs, r.edge_w));
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(512, tiles), cdiv(p->rows, 256)));
+  r.r_split = std::max<int64_t>(64, cdiv(cdiv(p->rows, splits), 64) * 64);
+  r.splits = (int)std::max<int64_t>(1, cdiv(p->rows, r.r_split));
+  // dz: blocks of 256 columns, about 2048 of them
+  const int64_t cols = std::max<int64_t>(1, cdiv(p->outputs, 256));
+  r.rows = (int)std::max<int64_t>(8, cdiv(cdiv(p->rows * cols, 2048), 8) * 8);
+  r.parts = (int)std::max<int64_t>(1, cdiv(p->rows, r.rows));
+  auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
+  r.dz = p->act == MRL_ACT_NONE ? 0 : up(p->rows * p->outputs * es);
+  r.part = up((int64_t)r.parts * p->outputs * 4);
+  r.slab = r.splits > 1 ? up((int64_t)r.splits * p->outputs * p->inputs * 4) : 0;
+  r.total = r.dz + r.part + r.slab;
+  return r;
+}
+
+template <typename T>
+int forward(const mrl_linear* p, const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, hipStream_t st) {
+  MmP a{};
+  a.a = x; a.lda = p->x_stride; a.b = w; a.ldb = p->inputs; a.M = (int)p->rows; a.N = p->outputs; a.R = p->inputs; a.r_split = std::max(p->inputs, 1);
+  a.y = y; a.bias = bias; a.residual = residual; a.z = z; a.act = p->act;
+  multiply<T, LAY_K, LAY_K>(a, edge_of(p->rows, p->outputs), 1, st);
+  return MRL_OK;
+}
+
+template <typename T>
+int backward(const mrl_linear* p, const void* x, const void* w, const void* z, const void* dy, void* dx, void* dw, void* db, char* ws, hipStream_t st) {
+  const Plan r = plan_of(p);
+  T* dz = reinterpret_cast<T*>(ws);
+  float* part = reinterpret_cast<float*>(ws + r.dz);
+  float* slab = reinterpret_cast<float*>(ws + r.dz + r.part);
+  const bool act = p->act != MRL_ACT_NONE;
+  if (p->rows > 0 && (db || (act && (dx || dw))))
+    hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)cdiv(p->outputs, 256), r.parts), dim3(256), 0, st, act ? static_cast<const T*>(z) : nullptr, static_cast<const T*>(dy),
+                       dz, db ? part : nullptr, p->rows, p->outputs, p->act, r.rows);
+  if (db) hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)cdiv(p->outputs, 32)), dim3(1024), 0, st, part, p->rows > 0 ? r.parts : 0, p->outputs, static_cast<T*>(db));
+  const void* d = act ? static_cast<const void*>(dz) : dy;
+  if (dx && p->rows > 0 && p->inputs > 0) {
+    MmP a{};
+    a.a = d; a.lda = p->outputs; a.b = w; a.ldb = p->inputs; a.M = (int)p->rows; a.N = p->inputs; a.R = p->outputs; a.r_split = p->outputs; a.y = dx;
+    multiply<T, LAY_K, LAY_R>(a, r.edge_x, 1, st);
+  }
+  if (dw && p->inputs > 0) {
+    MmP a{};
+    a.a = d; a.lda = p->outputs; a.b = x; a.ldb = p->x_stride; a.M = p->outputs; a.N = p->inputs; a.R = p->rows; a.r_split = r.r_split;
+    if (r.splits > 1) a.slab = slab;
+    else a.y = dw;
+    multiply<T, LAY_R, LAY_R>(a, r.edge_w, r.splits, st);
+    const int64_t n = (int64_t)p->outputs * p->inputs;
+    if (r.splits > 1) hipLaunchKernelGGL((slab_sum_kernel<T>), dim3((unsigned)cdiv(n, 1024)), dim3(256), 0, st, slab, r.splits, n, static_cast<T*>(dw));
+  }
+  return MRL_OK;
+}
+
+}  // namespace
+
+extern "C" int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, void* stream) {
+  const char* what = "mrl_linear_act";
+  const int rc = check(p, what);
+  if (rc) return rc;
+  if (p->rows == 0 || p->outputs == 0) return MRL_OK;
+  if (!y || (p->inputs > 0 && (!x || !weight))) MEM_FAIL(MRL_EINVAL, "%s: null data", what);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p->dtype == MRL_F32) forward<float>(p, x, weight, bias, residual, y, z, st);
+  else if (p->dtype == MRL_BF16) forward<__bf16>(p, x, weight, bias, residual, y, z, st);
+  else forward<_Float16>(p, x, weight, bias, residual, y, z, st);
+  MEM_CHECK_LAUNCH(what);
+  return MRL_OK;
+}
+
+extern "C" int64_t mrl_linear_act_backward_workspace_bytes(const mrl_linear* p) {
+  const int rc = check(p, "mrl_linear_act_backward_workspace_bytes");
+  if (rc) return rc;
+  return plan_of(p).total;
+}
+
+extern "C" int mrl_linear_act_backward(const mrl_linear* p, const void* x, const void* weight, const void* z, const void* dy, void* dx, void* d_weight, void* d_bias,
+                                       void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "mrl_linear_act_backward";
+  const int rc = check(p, what);
+  if (rc) return rc;
+  if (p->outputs == 0) MEM_FAIL(MRL_EINVAL, "%s: no outputs", what);
+  if (p->rows > 0) {
+    if (!dy || (p->act != MRL_ACT_NONE && !z)) MEM_FAIL(MRL_EINVAL, "%s: null dy or z", what);
+    if (p->inputs > 0 && ((dx && !weight) || (d_weight && !x))) MEM_FAIL(MRL_EINVAL, "%s: null x or weight", what);
+  }
+  const int64_t need = plan_of(p).total;
+  if (need > 0 && (!workspace || workspace_bytes < need)) MEM_FAIL(MRL_ENOSPC, "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
+  if ((uintptr_t)workspace & 15) MEM_FAIL(MRL_EINVAL, "%s: workspace is not aligned", what);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  if (p->dtype == MRL_F32) backward<float>(p, x, weight, z, dy, dx, d_weight, d_bias, ws, st);
+  else if (p->dtype == MRL_BF16) backward<__bf16>(p, x, weight, z, dy, dx, d_weight, d_bias, ws, st);
+  else backward<_Float16>(p, x, weight, z, dy, dx, d_weight, d_bias, ws, st);
+  MEM_CHECK_LAUNCH(what);
+  return MRL_OK;
+}

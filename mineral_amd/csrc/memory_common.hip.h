@@ -33,6 +33,67 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
 __device__ __forceinline__ float half_lo(unsigned pk) { return __uint_as_float(pk << 16); }
 __device__ __forceinline__ float half_hi(unsigned pk) { return __uint_as_float(pk & 0xffff0000u); }
 
+// Activations and their derivatives at z, in fp32.  `act` is uniform over the launch.  The logistic function uses the hardware's
+// exp2 and reciprocal (one spacing each); where a difference cancels near zero (ELU, tanh, erf) the library's functions do.
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+template <int N> __device__ __forceinline__ void act_fwd(int act, float (&z)[N]) {
+  switch (act) {
+    case MRL_ACT_SILU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) z[e] *= logistic(z[e]);
+      break;
+    case MRL_ACT_ELU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) z[e] = z[e] > 0.0f ? z[e] : expm1f(z[e]);
+      break;
+    case MRL_ACT_RELU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) z[e] = z[e] < 0.0f ? 0.0f : z[e];
+      break;
+    case MRL_ACT_TANH:
+#pragma unroll
+      for (int e = 0; e < N; ++e) z[e] = tanhf(z[e]);
+      break;
+    case MRL_ACT_GELU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) z[e] *= 0.5f * erfcf(z[e] * -0.70710678f);
+      break;
+    default: break;
+  }
+}
+// d[e] *= act'(z[e])
+template <int N> __device__ __forceinline__ void act_bwd(int act, const float (&z)[N], float (&d)[N]) {
+  switch (act) {
+    case MRL_ACT_SILU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float s = logistic(z[e]);
+        d[e] *= s * (1.0f + z[e] * (1.0f - s));
+      }
+      break;
+    case MRL_ACT_ELU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] *= z[e] > 0.0f ? 1.0f : expf(z[e]);
+      break;
+    case MRL_ACT_RELU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] = z[e] <= 0.0f ? 0.0f : d[e];
+      break;
+    case MRL_ACT_TANH:
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float t = tanhf(z[e]);
+        d[e] *= (1.0f - t) * (1.0f + t);
+      }
+      break;
+    case MRL_ACT_GELU:
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] *= 0.5f * erfcf(z[e] * -0.70710678f) + z[e] * 0.39894228f * expf(-0.5f * z[e] * z[e]);
+      break;
+    default: break;
+  }
+}
+
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 }  // namespace mem
 }  // namespace mrl

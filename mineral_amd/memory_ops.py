@@ -3,6 +3,10 @@
     import mineral_amd.ops
     o, state = torch.ops.mineral.linear_attention(q, k, v, log_decay, resets, initial_state, scale)      # a rollout, a prompt
     o = torch.ops.mineral.linear_attention_step(q, k, v, log_decay, state, resets, scale)                # one token, acting
+    y = torch.ops.mineral.group_norm_act(x, num_groups, weight, bias, eps, act_type)                     # channels last
+    y = torch.ops.mineral.linear_act(x, weight, bias, residual, act_type)                                # act(x W^T + b) + residual
+
+`act_type` is a name of the towers' configuration (None, 'SiLU', 'ELU', 'ReLU', 'Tanh') or 'GELU'.
 
 Registered for the device key only, like the operators of ops.py: CPU tensors fail in the dispatcher.  Tensors keep their type
 (float32, bfloat16 or float16); states are float32.  Calls run on the current stream of the tensors' device, whichever device is
@@ -167,10 +171,191 @@ def _linear_attention_step(q, k, v, log_decay, state, resets=None, scale=1.0):
     return out
 
 
+def _act(what, act_type):
+    if act_type not in _hip.ACT_TYPES:
+        raise NotImplementedError(f'{what}: act_type={act_type!r} (built: {", ".join(str(n) for n in _hip.ACT_TYPES)})')
+    return _hip.ACT_TYPES[act_type]
+
+
+def _aligned(t):
+    """Contiguous, on a 16-byte address."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+# ---- group norm ----------------------------------------------------------------------------------------------------------------
+def _group_norm(what, x, num_groups, weight, bias, eps, act_type):
+    """Checks of the arguments and their description."""
+    _require(x.dtype in _DTYPES, what, f'dtype {x.dtype} (float32, bfloat16 or float16)')
+    _require(x.dim() >= 2, what, f'x [batch, ..., channels], got {tuple(x.shape)}')
+    C_ = x.shape[-1]
+    _require(num_groups >= 1 and C_ >= 1 and C_ % num_groups == 0, what, f'{C_} channels are not {num_groups} groups')
+    _require(eps >= 0.0, what, f'eps {eps}')
+    _same_device(what, x, weight, bias)
+    pdt = x.dtype
+    for n, t in (('weight', weight), ('bias', bias)):
+        if t is not None:
+            _require(t.shape == (C_,) and t.dtype in (x.dtype, torch.float32), what, f'{n}: [{C_}] of {x.dtype} or float32, got {t.dtype} {tuple(t.shape)}')
+            pdt = t.dtype
+    _require(weight is None or bias is None or weight.dtype == bias.dtype, what, 'weight and bias of one type')
+    pixels = 1
+    for n in x.shape[1:-1]:
+        pixels *= n
+    return _hip.GroupNorm(x.shape[0], pixels, C_, num_groups, _DTYPES[x.dtype], _DTYPES[pdt], _act(what, act_type), eps), pdt
+
+
+def _norm_workspace(what, a, backward, like):
+    n = int(_hip.lib().mrl_group_norm_act_workspace_bytes(a, backward))
+    if n < 0:
+        _hip.check(n, what)
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None, n
+
+
+def _group_norm_forward(x, num_groups, weight, bias, eps, act_type, keep):
+    what = 'group_norm_act'
+    a, _ = _group_norm(what, x, num_groups, weight, bias, eps, act_type)
+    x = _aligned(x)
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, a.batch, num_groups), dtype=torch.float32, device=x.device) if keep else None
+    ws, n = _norm_workspace(what, a, 0, x)
+    with _on(x):
+        _hip.check(_hip.lib().mrl_group_norm_act(a, x.data_ptr(), _p(weight), _p(bias), y.data_ptr(), _p(stats[0]) if keep else None, _p(stats[1]) if keep else None,
+                                                 _p(ws), n, _stream(x)), what)
+    return y, stats
+
+
+def _group_norm_backward(dy, x, stats, num_groups, weight, bias, eps, act_type, need_params):
+    what = 'group_norm_act_backward'
+    a, pdt = _group_norm(what, x, num_groups, weight, bias, eps, act_type)
+    x, dy = _aligned(x), _aligned(dy)
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.numel() == 0:
+        return dx, *((torch.zeros(a.channels, dtype=pdt, device=x.device) for _ in range(2)) if need_params else (None, None))
+    dw, db = (torch.empty(a.channels, dtype=pdt, device=x.device) if need_params else None for _ in range(2))
+    ws, n = _norm_workspace(what, a, 1, x)
+    with _on(x):
+        _hip.check(_hip.lib().mrl_group_norm_act_backward(a, x.data_ptr(), dy.data_ptr(), _p(weight), _p(bias), stats[0].data_ptr(), stats[1].data_ptr(),
+                                                          dx.data_ptr(), _p(dw), _p(db), _p(ws), n, _stream(x)), what)
+    return dx, dw, db
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, num_groups, weight, bias, eps, act_type):
+        y, stats = _group_norm_forward(x, num_groups, weight, bias, eps, act_type, True)
+        ctx.save_for_backward(x, stats, weight, bias)
+        ctx.args = (num_groups, eps, act_type)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, stats, weight, bias = ctx.saved_tensors
+        num_groups, eps, act_type = ctx.args
+        n = ctx.needs_input_grad
+        dx, dw, db = _group_norm_backward(dy, x, stats, num_groups, weight, bias, eps, act_type, n[2] or n[3])
+        return dx, None, dw if n[2] else None, db if n[3] else None, None, None
+
+
+def _group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act_type=None):
+    return _group_norm_forward(x, num_groups, weight, bias, eps, act_type, False)[0]
+
+
+def _group_norm_act_autograd(x, num_groups, weight=None, bias=None, eps=1e-5, act_type=None):
+    if _wants_grad(x, weight, bias):
+        return _GroupNormAct.apply(x, num_groups, weight, bias, eps, act_type)
+    return _group_norm_forward(x, num_groups, weight, bias, eps, act_type, False)[0]
+
+
+# ---- linear layer ----------------------------------------------------------------------------------------------------------------
+def _linear(what, x, weight, bias, residual, act_type):
+    """Checks of the arguments; their description, and x as rows."""
+    _require(x.dtype in _DTYPES, what, f'dtype {x.dtype} (float32, bfloat16 or float16)')
+    _require(x.dim() >= 1 and weight.dim() == 2 and weight.shape[1] == x.shape[-1], what, f'x [.., inputs] and weight [outputs, inputs], got {tuple(x.shape)}, {tuple(weight.shape)}')
+    K, N = x.shape[-1], weight.shape[0]
+    _same_device(what, x, weight, bias, residual)
+    for n, t in (('weight', weight), ('bias', bias), ('residual', residual)):
+        _require(t is None or t.dtype == x.dtype, what, f'{n}: {x.dtype} like x, got {None if t is None else t.dtype}')
+    _require(bias is None or bias.shape == (N,), what, f'bias: [{N}], got {None if bias is None else tuple(bias.shape)}')
+    _require(residual is None or residual.shape == (*x.shape[:-1], N), what,
+             f'residual: {(*x.shape[:-1], N)}, got {None if residual is None else tuple(residual.shape)}; expand a broadcast one')
+    rows = 1
+    for n in x.shape[:-1]:
+        rows *= n
+    x = x.reshape(rows, K)
+    if K != 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < K:
+        x = x.contiguous()
+    return _hip.Linear(rows, x.stride(0) if rows > 1 else K, K, N, _DTYPES[x.dtype], _act(what, act_type)), x
+
+
+def _linear_forward(x, weight, bias, residual, act_type, keep):
+    what = 'linear_act'
+    a, rows = _linear(what, x, weight, bias, residual, act_type)
+    weight, bias, residual = (None if t is None else t.contiguous() for t in (weight, bias, residual))
+    shape = (*x.shape[:-1], a.outputs)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(shape, dtype=x.dtype, device=x.device) if keep and act_type is not None else None
+    with _on(x):
+        _hip.check(_hip.lib().mrl_linear_act(a, rows.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(z), _stream(x)), what)
+    return y, z
+
+
+def _linear_backward(dy, x, weight, z, act_type, needs):
+    what = 'linear_act_backward'
+    a, rows = _linear(what, x, weight, None, None, act_type)
+    need_x, need_w, need_b = needs
+    new = lambda shape, need: torch.empty(shape, dtype=x.dtype, device=x.device) if need else None  # noqa: E731
+    dx, dw, db = new(x.shape, need_x), new(weight.shape, need_w), new((a.outputs,), need_b)
+    if a.outputs == 0:
+        return None if dx is None else dx.zero_(), dw, db
+    weight, dy = weight.contiguous(), dy.contiguous()
+    n = int(_hip.lib().mrl_linear_act_backward_workspace_bytes(a))
+    if n < 0:
+        _hip.check(n, what)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    with _on(x):
+        _hip.check(_hip.lib().mrl_linear_act_backward(a, rows.data_ptr(), weight.data_ptr(), _p(z), dy.data_ptr(), _p(dx), _p(dw), _p(db), _p(ws), n, _stream(x)), what)
+    return dx, dw, db
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act_type):
+        y, z = _linear_forward(x, weight, bias, residual, act_type, True)
+        ctx.save_for_backward(x, weight, z)
+        ctx.act_type = act_type
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        n = ctx.needs_input_grad
+        dx = dw = db = None
+        if n[0] or n[1] or n[2]:
+            dx, dw, db = _linear_backward(dy, x, weight, z, ctx.act_type, n[:3])
+        return dx, dw, db, dy if n[3] else None, None
+
+
+def _linear_act(x, weight, bias=None, residual=None, act_type=None):
+    return _linear_forward(x, weight, bias, residual, act_type, False)[0]
+
+
+def _linear_act_autograd(x, weight, bias=None, residual=None, act_type=None):
+    if _wants_grad(x, weight, bias, residual):
+        return _LinearAct.apply(x, weight, bias, residual, act_type)
+    return _linear_forward(x, weight, bias, residual, act_type, False)[0]
+
+
 _lib.define('linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? resets=None, Tensor? initial_state=None, float scale=1.0) -> (Tensor, Tensor)')
 _lib.define('linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, Tensor? resets=None, float scale=1.0) -> Tensor')
+_lib.define('group_norm_act(Tensor x, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, str? act_type=None) -> Tensor')
+_lib.define('linear_act(Tensor x, Tensor weight, Tensor? bias=None, Tensor? residual=None, str? act_type=None) -> Tensor')
 
-OPS = ('linear_attention', 'linear_attention_step')
-for _name, _fn, _auto in (('linear_attention', _linear_attention, _linear_attention_autograd), ('linear_attention_step', _linear_attention_step, _linear_attention_step)):
+OPS = ('linear_attention', 'linear_attention_step', 'group_norm_act', 'linear_act')
+for _name, _fn, _auto in (('linear_attention', _linear_attention, _linear_attention_autograd), ('linear_attention_step', _linear_attention_step, _linear_attention_step),
+                          ('group_norm_act', _group_norm_act, _group_norm_act_autograd), ('linear_act', _linear_act, _linear_act_autograd)):
     _lib.impl(_name, _fn, 'CUDA')
     _lib.impl(_name, _auto, 'AutogradCUDA')
