@@ -8,7 +8,15 @@ OBJDIR = mineral_amd/csrc/build
 OBJ = $(patsubst mineral_amd/csrc/%.hip,$(OBJDIR)/%.o,$(SRC))
 LIB = mineral_amd/libmineral_ppo.so
 
-all: $(LIB)
+# torch.ops.mineral.* of the memory operators: host code over the C ABI, built against the installed torch
+TORCH := $(shell python3 -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+TORCHLIB = mineral_amd/libmineral_torch.so
+
+all: $(LIB) $(TORCHLIB)
+
+$(TORCHLIB): mineral_amd/csrc/torch_ops.cpp include/mineral_memory.h include/mineral_ppo.h $(LIB)
+	g++ -O2 -fPIC -shared -std=c++17 -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -isystem $(TORCH)/include -isystem $(TORCH)/include/torch/csrc/api/include -isystem /opt/rocm/include $< -o $@ \
+	  -Lmineral_amd -l:libmineral_ppo.so -L$(TORCH)/lib -ltorch_cpu -ltorch_hip -lc10 -lc10_hip -Wl,-rpath,'$$ORIGIN'
 
 $(LIB): $(OBJ)
 	$(HIPCC) $(HIPFLAGS) $(OBJ) -o $@
@@ -37,5 +45,5 @@ probes:
 	mkdir -p tools/bin && for p in $(PROBES); do $(HIPCC) --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops tools/$$p.hip -o tools/bin/$$p || exit 1; done
 
 clean:
-	rm -f $(LIB) $(OBJ)
+	rm -f $(LIB) $(TORCHLIB) $(OBJ)
 .PHONY: all resources ktrace ktrace-ablate probes clean

@@ -1,0 +1,429 @@
+// torch.ops.mineral.{linear_attention, linear_attention_step, group_norm_act, linear_act}: the operators of include/mineral_memory.h
+// as PyTorch operators with their gradients.  Host code only: checks of the arguments, allocation of outputs and workspaces through
+// torch's allocator, the launch on the current stream of the tensors' device.  In C++ because a call that acts for a few
+// environments takes less on the GPU than the interpreter needs to get there (17 us a call and 160 us for a call with its
+// gradient from Python on MI355X, measured with kernels of under 10 us).
+//
+// CPU tensors go through the same checks and are then refused: there is no CPU kernel.
+#include "../../include/mineral_memory.h"
+#include "../../include/mineral_ppo.h"
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <optional>
+#include <string>
+#include <tuple>
+
+namespace {
+
+using at::Tensor;
+using OptT = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+#define NEED(what, ok, ...) TORCH_CHECK_VALUE(ok, what, ": ", __VA_ARGS__)
+
+const Tensor none;
+const Tensor& of(const OptT& t) { return t.has_value() ? *t : none; }
+OptT opt(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+
+int dtype_of(const char* what, const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return MRL_F32;
+    case at::kBFloat16: return MRL_BF16;
+    case at::kHalf: return MRL_F16;
+    default: TORCH_CHECK_VALUE(false, what, ": dtype ", t.scalar_type(), " (float32, bfloat16 or float16)");
+  }
+}
+
+void same_device(const char* what, const Tensor& t, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* o : others) NEED(what, !o->defined() || o->device() == t.device(), "tensors on ", t.device(), " and ", o->device());
+}
+
+void check(int rc, const char* what) {
+  if (rc == MRL_OK) return;
+  const std::string msg = mrl_last_error();
+  TORCH_CHECK_VALUE(rc != MRL_EINVAL, what, ": ", msg);
+  TORCH_CHECK(false, what, " failed (", rc, "): ", msg);
+}
+
+const void* cp(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* mp(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+Tensor new_like(const Tensor& t, at::IntArrayRef shape) { return at::empty(shape, t.options().memory_format(at::MemoryFormat::Contiguous).requires_grad(false)); }
+Tensor new_floats(const Tensor& t, at::IntArrayRef shape) { return at::empty(shape, t.options().dtype(at::kFloat).requires_grad(false)); }
+
+struct Workspace {
+  Tensor t;
+  int64_t n;
+  Workspace(const char* what, int64_t bytes, const Tensor& like) : n(bytes) {
+    if (n < 0) check((int)n, what);
+    if (n > 0) t = at::empty({n}, like.options().dtype(at::kByte).requires_grad(false));
+  }
+  void* p() const { return mp(t); }
+};
+
+// the last dimension contiguous; every other stride stays
+Tensor rows_of(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+// contiguous, on a 16-byte address
+Tensor aligned(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return (reinterpret_cast<uintptr_t>(c.const_data_ptr()) & 15) ? c.clone() : c;
+}
+Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+void once(const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, ": differentiable once; its gradient under create_graph=True has none of its own");
+}
+
+[[noreturn]] void no_cpu(const char* what) { TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": tensors have to be on the GPU, there is no CPU kernel"); }
+
+// ---- linear attention ------------------------------------------------------------------------------------------------------------
+struct Attention {
+  mrl_attention a;
+  Tensor q, k, v, log_decay, resets, state;   // what `a` points into
+
+  Attention(const char* what, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& l_, const Tensor& r_, const Tensor& s_, double scale, bool step) {
+    a.dtype = dtype_of(what, q_);
+    NEED(what, k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type(), "q, k and v of one type, got ", q_.scalar_type(), ", ", k_.scalar_type(), ", ",
+         v_.scalar_type());
+    const int64_t dims = step ? 3 : 4;
+    bool ok = q_.dim() == dims && k_.sizes() == q_.sizes() && v_.dim() == dims;
+    for (int64_t i = 0; ok && i + 1 < dims; ++i) ok = v_.size(i) == q_.size(i);
+    NEED(what, ok, "q and k [batch, ", step ? "" : "steps, ", "heads, dim_k] and v [.., dim_v], got ", q_.sizes(), ", ", k_.sizes(), ", ", v_.sizes());
+    same_device(what, q_, {&k_, &v_, &l_, &r_, &s_});
+    a.batch = q_.size(0);
+    a.steps = step ? 1 : q_.size(1);
+    const int64_t H = q_.size(-2), K = q_.size(-1), V = v_.size(-1);
+    NEED(what, H >= 1 && H < (1 << 30) && K >= 1 && K <= MRL_ATTENTION_MAX_DIM && V >= 1 && V <= MRL_ATTENTION_MAX_DIM, H, " heads of dim_k ", K, ", dim_v ", V, " (1..",
+         MRL_ATTENTION_MAX_DIM, " each)");
+    a.heads = (int32_t)H; a.dim_k = (int32_t)K; a.dim_v = (int32_t)V;
+    NEED(what, l_.scalar_type() == at::kFloat && l_.dim() == 1 && l_.size(0) == H, "log_decay: float32 [", H, "], got ", l_.scalar_type(), " ", l_.sizes());
+    if (r_.defined()) {
+      const bool shape = step ? r_.dim() == 1 && r_.size(0) == a.batch : r_.dim() == 2 && r_.size(0) == a.batch && r_.size(1) == a.steps;
+      NEED(what, (r_.scalar_type() == at::kBool || r_.scalar_type() == at::kByte) && shape, "resets: bool or uint8 [batch", step ? "" : ", steps", "], got ", r_.scalar_type(),
+           " ", r_.sizes());
+      resets = r_.contiguous();
+    }
+    if (s_.defined()) {
+      NEED(what, s_.scalar_type() == at::kFloat && s_.dim() == 4 && s_.size(0) == a.batch && s_.size(1) == H && s_.size(2) == K && s_.size(3) == V,
+           "state: float32 [batch, heads, dim_k, dim_v], got ", s_.scalar_type(), " ", s_.sizes());
+      if (step) NEED(what, s_.is_contiguous(), "state is updated in place and has to be contiguous");
+      state = s_.contiguous();
+    }
+    q = rows_of(q_); k = rows_of(k_); v = rows_of(v_);
+    log_decay = l_.contiguous();
+    const Tensor* t[3] = {&q, &k, &v};
+    int64_t* st[3] = {a.q_stride, a.k_stride, a.v_stride};
+    for (int i = 0; i < 3; ++i) {
+      st[i][0] = t[i]->stride(0);
+      st[i][1] = step ? 0 : t[i]->stride(1);
+      st[i][2] = t[i]->stride(-2);
+    }
+    a.q = cp(q); a.k = cp(k); a.v = cp(v);
+    a.log_decay = static_cast<const float*>(cp(log_decay));
+    a.resets = static_cast<const uint8_t*>(cp(resets));
+    a.initial_state = step ? nullptr : static_cast<const float*>(cp(state));
+    a.scale = (float)scale;
+  }
+  Tensor new_state() const { return new_floats(q, {a.batch, a.heads, a.dim_k, a.dim_v}); }
+};
+
+std::tuple<Tensor, Tensor> attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& r, const Tensor& s, double scale) {
+  const char* what = "linear_attention";
+  const Attention d(what, q, k, v, l, r, s, scale, false);
+  c10::DeviceGuard guard(q.device());
+  Tensor out = new_like(v, v.sizes()), final = d.new_state();
+  const Workspace ws(what, mrl_linear_attention_workspace_bytes(&d.a, 0), q);
+  check(mrl_linear_attention(&d.a, mp(out), static_cast<float*>(mp(final)), ws.p(), ws.n, stream_of(q)), what);
+  return {out, final};
+}
+
+struct LinearAttention : Function<LinearAttention> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale,
+                               int64_t needs) {
+    ctx->set_materialize_grads(false);
+    auto [out, final] = attention_forward(q, k, v, l, of(r), of(s), scale);
+    ctx->save_for_backward({q, k, v, l, of(r), of(s)});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["needs"] = needs;
+    return {out, final};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const char* what = "linear_attention_backward";
+    once("linear_attention");
+    variable_list res(8);
+    if (!g[0].defined() && !g[1].defined()) return res;
+    const auto t = ctx->get_saved_variables();
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    const Attention d(what, t[0], t[1], t[2], t[3], t[4], t[5], ctx->saved_data["scale"].toDouble(), false);
+    c10::DeviceGuard guard(t[0].device());
+    const Tensor dout = g[0].defined() ? rows_of(g[0]) : at::zeros_like(t[2], at::MemoryFormat::Contiguous), dfinal = contiguous(g[1]);
+    const int64_t st[3] = {dout.stride(0), dout.stride(1), dout.stride(2)};
+    if (needs & 1) res[0] = new_like(t[0], t[0].sizes());
+    if (needs & 2) res[1] = new_like(t[1], t[1].sizes());
+    Tensor dv = needs & 12 ? new_like(t[2], t[2].sizes()) : Tensor();     // the state's gradient comes with it
+    if (needs & 4) res[2] = dv;
+    if (needs & 8) res[5] = d.new_state();
+    const Workspace ws(what, mrl_linear_attention_workspace_bytes(&d.a, 1), t[0]);
+    check(mrl_linear_attention_backward(&d.a, cp(dout), st, static_cast<const float*>(cp(dfinal)), mp(res[0]), mp(res[1]), mp(dv), static_cast<float*>(mp(res[5])), ws.p(),
+                                        ws.n, stream_of(t[0])), what);
+    return res;
+  }
+};
+
+std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale) {
+  return attention_forward(q, k, v, l, of(r), of(s), scale);
+}
+std::tuple<Tensor, Tensor> linear_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale) {
+  if (!wants_grad({&q, &k, &v, &l, &of(s)})) return attention_forward(q, k, v, l, of(r), of(s), scale);
+  TORCH_CHECK_NOT_IMPLEMENTED(!l.requires_grad(), "linear_attention: the decays are constants of the heads; log_decay has no gradient");
+  const int64_t needs = q.requires_grad() | k.requires_grad() << 1 | v.requires_grad() << 2 | (of(s).defined() && s->requires_grad()) << 3;
+  const auto o = LinearAttention::apply(q, k, v, l, r, s, scale, needs);
+  return {o[0], o[1]};
+}
+std::tuple<Tensor, Tensor> linear_attention_cpu(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale) {
+  const Attention d("linear_attention", q, k, v, l, of(r), of(s), scale, false);
+  no_cpu("linear_attention");
+}
+
+Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
+  const char* what = "linear_attention_step";
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({&q, &k, &v, &l, &state}), what, ": no gradient (linear_attention over the rollout has one); call it under torch.no_grad()");
+  const Attention d(what, q, k, v, l, of(r), state, scale, true);
+  if (q.is_cpu()) no_cpu(what);
+  c10::DeviceGuard guard(q.device());
+  Tensor out = new_like(v, v.sizes());
+  check(mrl_linear_attention_step(&d.a, static_cast<float*>(mp(state)), mp(out), stream_of(q)), what);
+  return out;
+}
+Tensor linear_attention_step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
+  state.unsafeGetTensorImpl()->bump_version();                            // written below torch's own bookkeeping
+  return linear_attention_step(q, k, v, l, state, r, scale);
+}
+
+// ---- activations -------------------------------------------------------------------------------------------------------------------
+int act_of(const char* what, const std::optional<std::string_view>& name) {
+  if (!name.has_value()) return MRL_ACT_NONE;
+  static constexpr std::pair<std::string_view, int> known[] = {{"SiLU", MRL_ACT_SILU}, {"ELU", MRL_ACT_ELU}, {"ReLU", MRL_ACT_RELU}, {"Tanh", MRL_ACT_TANH}, {"GELU", MRL_ACT_GELU}};
+  for (const auto& k : known)
+    if (*name == k.first) return k.second;
+  TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": act_type=", std::string(*name), " (built: None, SiLU, ELU, ReLU, Tanh, GELU)");
+}
+
+// ---- group norm ----------------------------------------------------------------------------------------------------------------------
+mrl_group_norm norm_of(const char* what, const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, double eps, int act) {
+  mrl_group_norm p;
+  p.dtype = dtype_of(what, x);
+  NEED(what, x.dim() >= 2, "x [batch, ..., channels], got ", x.sizes());
+  const int64_t C = x.size(-1);
+  NEED(what, groups >= 1 && C >= 1 && C <= (1 << 24) && C % groups == 0, C, " channels are not ", groups, " groups");
+  NEED(what, eps >= 0.0, "eps ", eps);
+  same_device(what, x, {&w, &b});
+  p.param_dtype = p.dtype;
+  for (const Tensor* t : {&w, &b})
+    if (t->defined()) {
+      NEED(what, t->dim() == 1 && t->size(0) == C && (t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat), "weight and bias: [", C, "] of ", x.scalar_type(),
+           " or float32, got ", t->scalar_type(), " ", t->sizes());
+      p.param_dtype = dtype_of(what, *t);
+    }
+  NEED(what, !w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight and bias of one type");
+  p.batch = x.size(0);
+  p.pixels = 1;
+  for (int64_t i = 1; i + 1 < x.dim(); ++i) p.pixels *= x.size(i);
+  p.channels = (int32_t)C; p.groups = (int32_t)groups; p.act = act; p.eps = (float)eps;
+  return p;
+}
+
+std::tuple<Tensor, Tensor> norm_forward(const Tensor& x_, int64_t groups, const Tensor& w_, const Tensor& b_, double eps, int act, bool keep) {
+  const char* what = "group_norm_act";
+  const mrl_group_norm p = norm_of(what, x_, groups, w_, b_, eps, act);
+  c10::DeviceGuard guard(x_.device());
+  const Tensor x = aligned(x_), w = contiguous(w_), b = contiguous(b_);
+  Tensor y = new_like(x, x.sizes()), stats = keep ? new_floats(x, {2, p.batch, groups}) : Tensor();
+  const Workspace ws(what, mrl_group_norm_act_workspace_bytes(&p, 0), x);
+  float* mean = keep ? static_cast<float*>(mp(stats)) : nullptr;
+  check(mrl_group_norm_act(&p, cp(x), cp(w), cp(b), mp(y), mean, keep ? mean + p.batch * groups : nullptr, ws.p(), ws.n, stream_of(x)), what);
+  return {y, stats};
+}
+
+struct GroupNormAct : Function<GroupNormAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptT& w, const OptT& b, int64_t groups, double eps, int64_t act, int64_t needs) {
+    auto [y, stats] = norm_forward(x, groups, of(w), of(b), eps, (int)act, true);
+    ctx->save_for_backward({x, stats, of(w), of(b)});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["needs"] = needs;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const char* what = "group_norm_act_backward";
+    once("group_norm_act");
+    const auto t = ctx->get_saved_variables();
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    const mrl_group_norm p = norm_of(what, t[0], ctx->saved_data["groups"].toInt(), t[2], t[3], ctx->saved_data["eps"].toDouble(), (int)ctx->saved_data["act"].toInt());
+    c10::DeviceGuard guard(t[0].device());
+    const Tensor x = aligned(t[0]), dy = aligned(g[0]), w = contiguous(t[2]), b = contiguous(t[3]);
+    Tensor dx = new_like(x, x.sizes()), dw, db;
+    if (needs & 6) {
+      const auto o = x.options().dtype(p.param_dtype == MRL_F32 ? at::kFloat : x.scalar_type()).requires_grad(false);
+      const bool empty = x.numel() == 0;
+      dw = empty ? at::zeros({p.channels}, o) : at::empty({p.channels}, o);
+      db = empty ? at::zeros({p.channels}, o) : at::empty({p.channels}, o);
+    }
+    if (x.numel() > 0) {
+      const Workspace ws(what, mrl_group_norm_act_workspace_bytes(&p, 1), x);
+      const float* mean = static_cast<const float*>(cp(t[1]));
+      check(mrl_group_norm_act_backward(&p, cp(x), cp(dy), cp(w), cp(b), mean, mean + p.batch * p.groups, mp(dx), mp(dw), mp(db), ws.p(), ws.n, stream_of(x)), what);
+    }
+    variable_list res(7);
+    res[0] = dx;
+    if (needs & 2) res[1] = dw;
+    if (needs & 4) res[2] = db;
+    return res;
+  }
+};
+
+using Name = std::optional<std::string_view>;
+
+Tensor group_norm_act(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
+  return std::get<0>(norm_forward(x, groups, of(w), of(b), eps, act_of("group_norm_act", act), false));
+}
+Tensor group_norm_act_autograd(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
+  if (!wants_grad({&x, &of(w), &of(b)})) return group_norm_act(x, groups, w, b, eps, act);
+  const int64_t needs = x.requires_grad() | (of(w).defined() && w->requires_grad()) << 1 | (of(b).defined() && b->requires_grad()) << 2;
+  return GroupNormAct::apply(x, w, b, groups, eps, (int64_t)act_of("group_norm_act", act), needs);
+}
+Tensor group_norm_act_cpu(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
+  norm_of("group_norm_act", x, groups, of(w), of(b), eps, act_of("group_norm_act", act));
+  no_cpu("group_norm_act");
+}
+
+// ---- linear layer ----------------------------------------------------------------------------------------------------------------------
+struct Linear {
+  mrl_linear p;
+  Tensor x;       // as rows
+
+  Linear(const char* what, const Tensor& x_, const Tensor& w, const Tensor& b, const Tensor& r, int act) {
+    p.dtype = dtype_of(what, x_);
+    NEED(what, x_.dim() >= 1 && w.dim() == 2 && w.size(1) == x_.size(-1), "x [.., inputs] and weight [outputs, inputs], got ", x_.sizes(), ", ", w.sizes());
+    const int64_t K = x_.size(-1), N = w.size(0);
+    same_device(what, x_, {&w, &b, &r});
+    const std::pair<const char*, const Tensor*> named[] = {{"weight", &w}, {"bias", &b}, {"residual", &r}};
+    for (const auto& n : named)
+      NEED(what, !n.second->defined() || n.second->scalar_type() == x_.scalar_type(), n.first, ": ", x_.scalar_type(), " like x, got ", n.second->scalar_type());
+    NEED(what, K <= (1 << 24) && N <= (1 << 24), "weight of ", w.sizes());
+    NEED(what, !b.defined() || (b.dim() == 1 && b.size(0) == N), "bias: [", N, "], got ", b.sizes());
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < x_.dim(); ++i) rows *= x_.size(i);
+    bool same = !r.defined() || (r.dim() == x_.dim() && r.size(-1) == N);
+    for (int64_t i = 0; same && r.defined() && i + 1 < x_.dim(); ++i) same = r.size(i) == x_.size(i);
+    NEED(what, same, "residual: the output's shape, got ", r.sizes(), " beside x ", x_.sizes(), " and ", N, " outputs; expand a broadcast one");
+    x = x_.dim() == 2 ? x_ : x_.reshape({rows, K});
+    if ((K != 1 && x.stride(1) != 1) || (rows > 1 && x.stride(0) < K)) x = x.contiguous();
+    p.rows = rows; p.x_stride = rows > 1 ? x.stride(0) : K;
+    p.inputs = (int32_t)K; p.outputs = (int32_t)N; p.act = act;
+  }
+  at::DimVector out_shape(const Tensor& x_) const {
+    at::DimVector s(x_.sizes().begin(), x_.sizes().end());
+    s.back() = p.outputs;
+    return s;
+  }
+};
+
+std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w_, const Tensor& b_, const Tensor& r_, int act, bool keep) {
+  const char* what = "linear_act";
+  const Linear d(what, x, w_, b_, r_, act);
+  c10::DeviceGuard guard(x.device());
+  const Tensor w = w_.contiguous(), b = contiguous(b_), r = contiguous(r_);
+  const auto shape = d.out_shape(x);
+  Tensor y = new_like(x, shape), z = keep && act != MRL_ACT_NONE ? new_like(x, shape) : Tensor();
+  check(mrl_linear_act(&d.p, cp(d.x), cp(w), cp(b), cp(r), mp(y), mp(z), stream_of(x)), what);
+  return {y, z};
+}
+
+struct LinearAct : Function<LinearAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, int64_t act, int64_t needs) {
+    auto [y, z] = linear_forward(x, w, of(b), of(r), (int)act, needs & 7);
+    ctx->save_for_backward({x, w, z});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["needs"] = needs;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const char* what = "linear_act_backward";
+    once("linear_act");
+    variable_list res(6);
+    const int64_t needs = ctx->saved_data["needs"].toInt();
+    if (needs & 8) res[3] = g[0];
+    if (!(needs & 7)) return res;
+    const auto t = ctx->get_saved_variables();
+    const Linear d(what, t[0], t[1], none, none, (int)ctx->saved_data["act"].toInt());
+    c10::DeviceGuard guard(t[0].device());
+    if (needs & 1) res[0] = new_like(t[0], t[0].sizes());
+    if (needs & 2) res[1] = new_like(t[1], t[1].sizes());
+    if (needs & 4) res[2] = new_like(t[0], {d.p.outputs});
+    if (d.p.outputs == 0) {
+      if (res[0].defined()) res[0].zero_();
+      return res;
+    }
+    const Tensor w = t[1].contiguous(), dy = g[0].contiguous();
+    const Workspace ws(what, mrl_linear_act_backward_workspace_bytes(&d.p), dy);
+    check(mrl_linear_act_backward(&d.p, cp(d.x), cp(w), cp(t[2]), cp(dy), mp(res[0]), mp(res[1]), mp(res[2]), ws.p(), ws.n, stream_of(dy)), what);
+    return res;
+  }
+};
+
+Tensor linear_act(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
+  return std::get<0>(linear_forward(x, w, of(b), of(r), act_of("linear_act", act), false));
+}
+Tensor linear_act_autograd(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
+  if (!wants_grad({&x, &w, &of(b), &of(r)})) return linear_act(x, w, b, r, act);
+  const int64_t needs = x.requires_grad() | w.requires_grad() << 1 | (of(b).defined() && b->requires_grad()) << 2 | (of(r).defined() && r->requires_grad()) << 3;
+  return LinearAct::apply(x, w, b, r, (int64_t)act_of("linear_act", act), needs);
+}
+Tensor linear_act_cpu(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
+  const Linear d("linear_act", x, w, of(b), of(r), act_of("linear_act", act));
+  no_cpu("linear_act");
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(mineral, m) {
+  m.def("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? resets=None, Tensor? initial_state=None, float scale=1.0) -> (Tensor, Tensor)");
+  m.def("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, Tensor? resets=None, float scale=1.0) -> Tensor");
+  m.def("group_norm_act(Tensor x, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, str? act_type=None) -> Tensor");
+  m.def("linear_act(Tensor x, Tensor weight, Tensor? bias=None, Tensor? residual=None, str? act_type=None) -> Tensor");
+}
+TORCH_LIBRARY_IMPL(mineral, CUDA, m) {
+  m.impl("linear_attention", linear_attention);
+  m.impl("linear_attention_step", linear_attention_step);
+  m.impl("group_norm_act", group_norm_act);
+  m.impl("linear_act", linear_act);
+}
+TORCH_LIBRARY_IMPL(mineral, AutogradCUDA, m) {
+  m.impl("linear_attention", linear_attention_autograd);
+  m.impl("linear_attention_step", linear_attention_step_autograd);
+  m.impl("group_norm_act", group_norm_act_autograd);
+  m.impl("linear_act", linear_act_autograd);
+}
+TORCH_LIBRARY_IMPL(mineral, CPU, m) {
+  m.impl("linear_attention", linear_attention_cpu);
+  m.impl("linear_attention_step", linear_attention_step);
+  m.impl("group_norm_act", group_norm_act_cpu);
+  m.impl("linear_act", linear_act_cpu);
+}

@@ -227,22 +227,27 @@ def test_nothing_to_do_and_refusals_on_the_device():
 
 
 def test_refusals():
-    from mineral_amd import _hip, memory_ops
+    """Argument checks, on CPU tensors: they come before the refusal of the CPU itself."""
+    from mineral_amd import _hip
     x, w, b, _ = make((4, 8), torch.float32, 7)
-    f = lambda **k: memory_ops._group_norm(**{**dict(what='t', x=x, num_groups=2, weight=w, bias=b, eps=1e-5, act_type=None), **k})  # noqa: E731
-    a, _ = f()
+    ok = dict(x=x, num_groups=2, weight=w, bias=b, eps=1e-5, act_type=None)
+    with pytest.raises(NotImplementedError, match='CPU'):
+        ops().group_norm_act(**ok)
+    with pytest.raises(NotImplementedError, match='act_type'):
+        ops().group_norm_act(**{**ok, 'act_type': 'Mish'})
     for change, text in ((dict(x=x.double()), 'dtype'), (dict(x=x[0]), 'channels'), (dict(num_groups=3), 'groups'), (dict(num_groups=0), 'groups'), (dict(eps=-1.0), 'eps'),
-                         (dict(weight=w[:4]), 'weight'), (dict(bias=b.half()), 'bias'), (dict(x=x.half(), weight=w.half()), 'one type')):
+                         (dict(eps=float('nan')), 'eps'), (dict(weight=w[:4]), 'weight'), (dict(bias=b.half()), 'bias'), (dict(x=x.half(), weight=w.half()), 'one type')):
         with pytest.raises(ValueError, match=text):
-            f(**change)
+            ops().group_norm_act(**{**ok, **change})
+    a = _hip.GroupNorm(4, 1, 8, 2, 0, 0, 0, 1e-5)
     L = _hip.lib()
     assert L.mrl_group_norm_act_workspace_bytes(a, 0) == 0 and L.mrl_group_norm_act_workspace_bytes(a, 1) > 0
     assert L.mrl_group_norm_act(a, None, None, None, None, None, None, None, 0, None) == -1 and b'null' in L.mrl_last_error()
     assert L.mrl_group_norm_act(None, None, None, None, None, None, None, None, 0, None) == -1
     assert L.mrl_group_norm_act(a, 4, None, None, 16, None, None, None, 0, None) == -1 and b'aligned' in L.mrl_last_error()
+    assert L.mrl_group_norm_act(a, 16, None, None, 16, 16, None, None, 0, None) == -1 and b'together' in L.mrl_last_error()
     assert L.mrl_group_norm_act_backward(a, 16, 16, None, None, 16, 16, 16, 16, 16, None, 0, None) == -2
     assert L.mrl_group_norm_act_backward(a, 16, 16, None, None, 16, 16, 16, 16, None, None, 0, None) == -1
-    a.act = 9
-    assert L.mrl_group_norm_act_workspace_bytes(a, 0) == -1
-    with pytest.raises(NotImplementedError):
-        ops().group_norm_act(x, 2, w, b, 1e-5, None)
+    for bad in (_hip.GroupNorm(4, 1, 8, 3, 0, 0, 0, 1e-5), _hip.GroupNorm(4, 1, 8, 2, 3, 0, 0, 1e-5), _hip.GroupNorm(4, 1, 8, 2, 1, 2, 0, 1e-5),
+                _hip.GroupNorm(4, 1, 8, 2, 0, 0, 9, 1e-5), _hip.GroupNorm(-1, 1, 8, 2, 0, 0, 0, 1e-5)):
+        assert L.mrl_group_norm_act_workspace_bytes(bad, 0) == -1

@@ -223,22 +223,27 @@ def test_offsets_beyond_32_bits():
 
 
 def test_refusals():
-    from mineral_amd import _hip, memory_ops
+    """Argument checks, on CPU tensors: they come before the refusal of the CPU itself."""
+    from mineral_amd import _hip
     x, w, b, r, _ = make(4, 8, 6, torch.float32, 10)
-    f = lambda **k: memory_ops._linear(**{**dict(what='t', x=x, weight=w, bias=b, residual=r, act_type=None), **k})  # noqa: E731
-    a, rows = f()
+    ok = dict(x=x, weight=w, bias=b, residual=r, act_type=None)
+    with pytest.raises(NotImplementedError, match='CPU'):
+        ops().linear_act(**ok)
+    with pytest.raises(NotImplementedError, match='act_type'):
+        ops().linear_act(**{**ok, 'act_type': 'Mish'})
     for change, text in ((dict(x=x.double()), 'dtype'), (dict(weight=w[:, :4]), 'weight'), (dict(weight=w[0]), 'weight'), (dict(weight=w.half()), 'weight'),
                          (dict(bias=b[:3]), 'bias'), (dict(bias=b.half()), 'bias'), (dict(residual=r[:1]), 'residual'), (dict(residual=r.half()), 'residual')):
         with pytest.raises(ValueError, match=text):
-            f(**change)
+            ops().linear_act(**{**ok, **change})
     L = _hip.lib()
+    a = _hip.Linear(4, 8, 8, 6, 0, 0)
     assert L.mrl_linear_act(a, None, None, None, None, None, None, None) == -1 and b'null' in L.mrl_last_error()
     assert L.mrl_linear_act(None, None, None, None, None, None, None, None) == -1
     assert L.mrl_linear_act_backward_workspace_bytes(a) > 0
     assert L.mrl_linear_act_backward(a, 16, 16, None, 16, 16, 16, 16, None, 0, None) == -2
     a.act = 1
-    assert L.mrl_linear_act_backward(a, 16, 16, None, 16, 16, 16, 16, 16, 1 << 30, None) == -1 and b'z' in L.mrl_last_error()
+    assert L.mrl_linear_act_backward(a, 16, 16, None, 16, 16, 16, 16, 16, 1 << 30, None) == -1
     a.x_stride = 3
     assert L.mrl_linear_act(a, 16, 16, None, None, 16, None, None) == -1 and b'x_stride' in L.mrl_last_error()
-    with pytest.raises(NotImplementedError):
-        ops().linear_act(x, w, b, r, None)
+    for bad in (_hip.Linear(4, 8, 8, 6, 3, 0), _hip.Linear(4, 8, 8, 6, 0, 6), _hip.Linear(-1, 8, 8, 6, 0, 0), _hip.Linear(4, 1 << 25, 1 << 25, 6, 0, 0)):
+        assert L.mrl_linear_act_backward_workspace_bytes(bad) == -1

@@ -358,34 +358,44 @@ def test_refusals_on_the_device():
 
 
 def test_refusals():
-    """Argument checks, without a GPU."""
-    from mineral_amd import _hip, memory_ops
+    """Argument checks, on CPU tensors: they come before the refusal of the CPU itself."""
+    from mineral_amd import _hip
+    M = ops()
     q, k, v, l, r, s = make(2, 4, 2, 8, 12, torch.float32, 18)
-    ok = dict(what='t', q=q, k=k, v=v, log_decay=l, resets=r, state=s, scale=1.0, step=False)
-    a, _ = memory_ops._attention(**ok)
-    L = _hip.lib()
-    assert L.mrl_linear_attention_workspace_bytes(a, 0) == 0
+    ok = dict(q=q, k=k, v=v, log_decay=l, resets=r, initial_state=s, scale=1.0)
+    with pytest.raises(NotImplementedError, match='CPU'):
+        M.linear_attention(**ok)
+    wide = torch.zeros(2, 4, 2, 129)
     for change, text in ((dict(q=q.double()), 'dtype'), (dict(k=k.half()), 'one type'), (dict(k=k[:, :3]), 'dim_k'), (dict(v=v[:1]), 'dim_v'),
                          (dict(log_decay=l[:1]), 'log_decay'), (dict(log_decay=l.double()), 'log_decay'), (dict(resets=r.float()), 'resets'),
-                         (dict(resets=r[:, :2]), 'resets'), (dict(state=s.half()), 'state'), (dict(state=s[:, :1]), 'state'), (dict(q=q[0]), 'dim_k')):
+                         (dict(resets=r[:, :2]), 'resets'), (dict(initial_state=s.half()), 'state'), (dict(initial_state=s[:, :1]), 'state'), (dict(q=q[0]), 'dim_k'),
+                         (dict(q=wide, k=wide), '128'), (dict(v=v[..., :0]), 'dim_v'), (dict(q=q[:, :, :0], k=k[:, :, :0], v=v[:, :, :0]), 'heads')):
         with pytest.raises(ValueError, match=text):
-            memory_ops._attention(**{**ok, **change})
-    with pytest.raises(NotImplementedError):                 # CPU tensors: refused by the dispatcher
-        ops().linear_attention(q, k, v, l, r, s, 1.0)
-    wide = torch.zeros(1, 2, 1, 129)
-    a, _ = memory_ops._attention('t', wide, wide, wide, torch.zeros(1), None, None, 1.0, False)
-    assert L.mrl_linear_attention_workspace_bytes(a, 0) == -1 and b'128' in L.mrl_last_error()
-    a, held = memory_ops._attention(**ok)
+            M.linear_attention(**{**ok, **change})
+    step = dict(q=q[:, 0], k=k[:, 0], v=v[:, 0], log_decay=l, state=s, resets=r[:, 0], scale=1.0)
+    with pytest.raises(NotImplementedError, match='CPU'):
+        M.linear_attention_step(**step)
+    for change, text in ((dict(state=s.transpose(2, 3).contiguous().transpose(2, 3)), 'in place'), (dict(state=s[:1]), 'state'), (dict(resets=r), 'resets'), (dict(q=q), 'dim_k')):
+        with pytest.raises(ValueError, match=text):
+            M.linear_attention_step(**{**step, **change})
+    # the C ABI
+    L = _hip.lib()
+    i3 = C.c_int64 * 3
+
+    def desc(B=2, T=4, H=2, K=8, V=12, dtype=0):
+        return _hip.Attention(B, T, H, K, V, dtype, 16, 16, 16, i3(T * H * K, H * K, K), i3(T * H * K, H * K, K), i3(T * H * V, H * V, V), 16, None, None, 1.0)
+    a = desc()
+    assert L.mrl_linear_attention_workspace_bytes(a, 0) == 0
+    for bad in (desc(K=129), desc(V=0), desc(H=0), desc(T=-1), desc(T=1 << 30), desc(B=1 << 30), desc(dtype=7)):
+        assert L.mrl_linear_attention_workspace_bytes(bad, 0) == -1
     assert L.mrl_linear_attention(a, None, None, None, 0, None) == -1 and b'null output' in L.mrl_last_error()
     assert L.mrl_linear_attention(None, None, None, None, 0, None) == -1
     assert L.mrl_linear_attention_step(a, None, None, None) == -1 and b'steps' in L.mrl_last_error()
     assert L.mrl_linear_attention_backward(a, None, None, None, None, None, None, None, None, 0, None) == -1
-    a.dtype = 7
-    assert L.mrl_linear_attention_workspace_bytes(a, 0) == -1
-    long = torch.empty(1, 4096, 1, 8)
-    a, held = memory_ops._attention('t', long, long, long, torch.zeros(1), None, None, 1.0, False)
-    assert L.mrl_linear_attention_workspace_bytes(a, 0) > 0
-    assert L.mrl_linear_attention(a, C.c_void_p(16), C.c_void_p(16), None, 0, None) == -2 and b'workspace' in L.mrl_last_error()
+    assert L.mrl_linear_attention_backward(a, 16, i3(0, 0, 0), None, 16, 16, None, 16, None, 0, None) == -1 and b'd_initial_state' in L.mrl_last_error()
+    long = desc(T=4096)
+    assert L.mrl_linear_attention_workspace_bytes(long, 0) > 0
+    assert L.mrl_linear_attention(long, 16, 16, None, 0, None) == -2 and b'workspace' in L.mrl_last_error()
 
 
 def test_header_and_binding_list_the_same_entry_points():
