@@ -91,14 +91,15 @@ typedef struct mrl_linear {
   int32_t inputs, outputs, dtype, act;
 } mrl_linear;
 
-/* z : [rows][outputs] of dtype or NULL: x W^T + bias, what the backward call reads where act is not MRL_ACT_NONE. */
-int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, void* stream);
+/* slope : [rows][outputs] or NULL: act'(x W^T + bias), what the backward call reads where act is not MRL_ACT_NONE: fp32 beside MRL_F32,
+ * otherwise 16 bits (sign, 4 bits of exponent, 11 of mantissa). */
+int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const void* bias, const void* residual, void* y, void* slope, void* stream);
 
 int64_t mrl_linear_act_backward_workspace_bytes(const mrl_linear* p);
 
 /* dx [rows][inputs], d_weight [outputs][inputs], d_bias [outputs], contiguous; a NULL output is not computed.  The residual's gradient
- * is dy itself.  dz = dy act'(z) is rounded to dtype before the products; d_bias sums it unrounded. */
-int mrl_linear_act_backward(const mrl_linear* p, const void* x, const void* weight, const void* z, const void* dy, void* dx, void* d_weight, void* d_bias,
+ * is dy itself.  dz = dy slope is rounded to dtype before the products; d_bias sums it unrounded.  A slope of zero drops dy, whatever it is. */
+int mrl_linear_act_backward(const mrl_linear* p, const void* x, const void* weight, const void* slope, const void* dy, void* dx, void* d_weight, void* d_bias,
                             void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

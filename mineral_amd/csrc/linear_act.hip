@@ -4,7 +4,7 @@
 // W forward, dz for dx) or with rows of the reduction index (W for dx, both for dW), and goes to LDS as it lies; fragments of the
 // first kind are 16-byte reads, of the second transposing reads.  Tiles travel HBM -> registers -> LDS one step ahead of the MFMAs.
 // The MFMAs take the operands swapped, so a lane's accumulators are four neighbouring columns of one row; the epilogue passes them
-// through LDS once and then works on rows: bias, z, activation, residual and stores in 16-byte units.
+// through LDS once and then works on rows: bias, activation and its slope, residual and stores in 16-byte units.
 // fp32 operands are split exactly into three bf16 terms on their way to LDS and multiply in six products, smallest first.
 // dW sums over all rows: they are split over blocks whose partial sums are added in a fixed order.
 #include "memory_common.hip.h"
@@ -27,7 +27,7 @@ struct MmP {
   void* y;                  // [M][N]
   float* slab;              // instead of y: [splits][M][N] fp32
   const void *bias, *residual;
-  void* z;
+  void* slope;              // act'(z): fp32, or packed to 16 bits beside 16-bit types
   int act;
 };
 
@@ -168,6 +168,44 @@ template <typename T, int N> __device__ __forceinline__ void store_row(T* p, int
   }
 }
 
+// An activation's slope (magnitude below 2) in 16 bits: sign, 4 bits of exponent, 11 of mantissa, rounded to nearest.  What the
+// backward pass needs of z, in z's room but 2^-12 relative at worst (2^-26 absolute below 2^-14): rounded z or slopes in bf16 or
+// fp16 would add as much error to the gradients as their own rounding.  All ones stand for NaN.
+__device__ __forceinline__ unsigned pack_slope(float s) {
+  const unsigned sign = (__float_as_uint(s) >> 16) & 0x8000u;
+  unsigned a = __float_as_uint(__builtin_fabsf(s) * 0x1p-112f);    // now the exponent fits 4 bits (subnormals included)
+  a = (a + 0x7ffu + ((a >> 12) & 1u)) >> 12;
+  return (__builtin_fabsf(s) < 1.9f ? a : 0x7fffu) | sign;
+}
+__device__ __forceinline__ float unpack_slope(unsigned u) {
+  const float a = __uint_as_float((u & 0x7fffu) << 12) * 0x1p112f;
+  return (u & 0x7fffu) == 0x7fffu ? __builtin_nanf("") : (u & 0x8000u) ? -a : a;
+}
+template <typename T> struct SlopeOf { typedef unsigned short S; };
+template <> struct SlopeOf<float> { typedef float S; };
+template <typename S> __device__ __forceinline__ void load_slopes(const S* p, int left, float (&x)[8]) {
+  if constexpr (sizeof(S) == 4) load_row<float, 8>(p, left, x);
+  else {
+    const u32x4 w = load_unit<__bf16>(reinterpret_cast<const __bf16*>(p), left);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = unpack_slope((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+  }
+}
+template <typename S> __device__ __forceinline__ void store_slopes(S* p, int left, const float (&x)[8]) {
+  if constexpr (sizeof(S) == 4) store_row<float, 8>(p, left, x);
+  else {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack_slope(x[2 * e]) | pack_slope(x[2 * e + 1]) << 16;
+    if (left >= 8) __builtin_memcpy(p, &w, 16);
+    else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) p[e] = (S)(w[e / 2] >> (16 * (e & 1)));
+    }
+  }
+}
+
 // WM x WN waves over the tile, WK waves over the reduction inside a step
 template <typename T, int BM, int BN, int BK, int WM, int WN, int WK, int LA, int LB, int NBUF>
 __global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
@@ -305,7 +343,12 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += b[e];
     }
-    if (p.z) store_row<T, 8>(static_cast<T*>(p.z) + at, left, v);
+    if (p.slope) {
+      typedef typename SlopeOf<T>::S S;
+      float d[8];
+      act_slope<8>(p.act, v, d);
+      store_slopes<S>(static_cast<S*>(p.slope) + at, left, d);
+    }
     act_fwd<8>(p.act, v);
     if (p.residual) {
       float b[8];
@@ -317,10 +360,10 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
   }
 }
 
-// dz = dy act'(z), and the sums of its columns over this block's rows -> part [blocks in y][N].  32 units of 8 columns x 8 rows a block.
+// dz = dy slope, and the sums of its columns over this block's rows -> part [blocks in y][N].  32 units of 8 columns x 8 rows a block.
 template <typename T>
-__global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ z, const T* __restrict__ dy, T* __restrict__ dz, float* __restrict__ part, int64_t M, int N, int act,
-                                                 int rows) {
+__global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* __restrict__ slope, const T* __restrict__ dy, T* __restrict__ dz, float* __restrict__ part,
+                                                 int64_t M, int N, int rows) {
   __shared__ float red[8][32 * 8 + 1];
   const int cu = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + cu) * 8, left = N - c;
@@ -330,11 +373,12 @@ __global__ __launch_bounds__(256) void dz_kernel(const T* __restrict__ z, const 
   if (left > 0) {
     const int64_t m1 = min(M, ((int64_t)blockIdx.y + 1) * rows);
     for (int64_t m = (int64_t)blockIdx.y * rows + rl; m < m1; m += 8) {
-      float d[8], zz[8];
+      float d[8], g[8];
       load_row<T, 8>(dy + m * N + c, left, d);
-      if (z) {
-        load_row<T, 8>(z + m * N + c, left, zz);
-        act_bwd<8>(act, zz, d);
+      if (slope) {
+        load_slopes(slope + m * N + c, left, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = g[e] == 0.0f ? 0.0f : d[e] * g[e];
         store_row<T, 8>(dz + m * N + c, left, d);
       }
 #pragma unroll
@@ -450,24 +494,24 @@ Plan plan_of(const mrl_linear* p) {
 }
 
 template <typename T>
-int forward(const mrl_linear* p, const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, hipStream_t st) {
+int forward(const mrl_linear* p, const void* x, const void* w, const void* bias, const void* residual, void* y, void* slope, hipStream_t st) {
   MmP a{};
   a.a = x; a.lda = p->x_stride; a.b = w; a.ldb = p->inputs; a.M = (int)p->rows; a.N = p->outputs; a.R = p->inputs; a.r_split = std::max(p->inputs, 1);
-  a.y = y; a.bias = bias; a.residual = residual; a.z = z; a.act = p->act;
+  a.y = y; a.bias = bias; a.residual = residual; a.slope = slope; a.act = p->act;
   multiply<T, LAY_K, LAY_K>(a, edge_of(p->rows, p->outputs), 1, st);
   return MRL_OK;
 }
 
 template <typename T>
-int backward(const mrl_linear* p, const void* x, const void* w, const void* z, const void* dy, void* dx, void* dw, void* db, char* ws, hipStream_t st) {
+int backward(const mrl_linear* p, const void* x, const void* w, const void* slope, const void* dy, void* dx, void* dw, void* db, char* ws, hipStream_t st) {
   const Plan r = plan_of(p);
   T* dz = reinterpret_cast<T*>(ws);
   float* part = reinterpret_cast<float*>(ws + r.dz);
   float* slab = reinterpret_cast<float*>(ws + r.dz + r.part);
   const bool act = p->act != MRL_ACT_NONE;
   if (p->rows > 0 && (db || (act && (dx || dw))))
-    hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)cdiv(p->outputs, 256), r.parts), dim3(256), 0, st, act ? static_cast<const T*>(z) : nullptr, static_cast<const T*>(dy),
-                       dz, db ? part : nullptr, p->rows, p->outputs, p->act, r.rows);
+    hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)cdiv(p->outputs, 256), r.parts), dim3(256), 0, st,
+                       act ? static_cast<const typename SlopeOf<T>::S*>(slope) : nullptr, static_cast<const T*>(dy), dz, db ? part : nullptr, p->rows, p->outputs, r.rows);
   if (db) hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)cdiv(p->outputs, 32)), dim3(1024), 0, st, part, p->rows > 0 ? r.parts : 0, p->outputs, static_cast<T*>(db));
   const void* d = act ? static_cast<const void*>(dz) : dy;
   if (dx && p->rows > 0 && p->inputs > 0) {
@@ -489,16 +533,16 @@ int backward(const mrl_linear* p, const void* x, const void* w, const void* z, c
 
 }  // namespace
 
-extern "C" int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, void* stream) {
+extern "C" int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const void* bias, const void* residual, void* y, void* slope, void* stream) {
   const char* what = "mrl_linear_act";
   const int rc = check(p, what);
   if (rc) return rc;
   if (p->rows == 0 || p->outputs == 0) return MRL_OK;
   if (!y || (p->inputs > 0 && (!x || !weight))) MEM_FAIL(MRL_EINVAL, "%s: null data", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p->dtype == MRL_F32) forward<float>(p, x, weight, bias, residual, y, z, st);
-  else if (p->dtype == MRL_BF16) forward<__bf16>(p, x, weight, bias, residual, y, z, st);
-  else forward<_Float16>(p, x, weight, bias, residual, y, z, st);
+  if (p->dtype == MRL_F32) forward<float>(p, x, weight, bias, residual, y, slope, st);
+  else if (p->dtype == MRL_BF16) forward<__bf16>(p, x, weight, bias, residual, y, slope, st);
+  else forward<_Float16>(p, x, weight, bias, residual, y, slope, st);
   MEM_CHECK_LAUNCH(what);
   return MRL_OK;
 }
@@ -509,14 +553,14 @@ extern "C" int64_t mrl_linear_act_backward_workspace_bytes(const mrl_linear* p) 
   return plan_of(p).total;
 }
 
-extern "C" int mrl_linear_act_backward(const mrl_linear* p, const void* x, const void* weight, const void* z, const void* dy, void* dx, void* d_weight, void* d_bias,
+extern "C" int mrl_linear_act_backward(const mrl_linear* p, const void* x, const void* weight, const void* slope, const void* dy, void* dx, void* d_weight, void* d_bias,
                                        void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "mrl_linear_act_backward";
   const int rc = check(p, what);
   if (rc) return rc;
   if (p->outputs == 0) MEM_FAIL(MRL_EINVAL, "%s: no outputs", what);
   if (p->rows > 0) {
-    if (!dy || (p->act != MRL_ACT_NONE && !z)) MEM_FAIL(MRL_EINVAL, "%s: null dy or z", what);
+    if (!dy || (p->act != MRL_ACT_NONE && !slope)) MEM_FAIL(MRL_EINVAL, "%s: null dy or slope", what);
     if (p->inputs > 0 && ((dx && !weight) || (d_weight && !x))) MEM_FAIL(MRL_EINVAL, "%s: null x or weight", what);
   }
   const int64_t need = plan_of(p).total;
@@ -524,9 +568,9 @@ extern "C" int mrl_linear_act_backward(const mrl_linear* p, const void* x, const
   if ((uintptr_t)workspace & 15) MEM_FAIL(MRL_EINVAL, "%s: workspace is not aligned", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  if (p->dtype == MRL_F32) backward<float>(p, x, weight, z, dy, dx, d_weight, d_bias, ws, st);
-  else if (p->dtype == MRL_BF16) backward<__bf16>(p, x, weight, z, dy, dx, d_weight, d_bias, ws, st);
-  else backward<_Float16>(p, x, weight, z, dy, dx, d_weight, d_bias, ws, st);
+  if (p->dtype == MRL_F32) backward<float>(p, x, weight, slope, dy, dx, d_weight, d_bias, ws, st);
+  else if (p->dtype == MRL_BF16) backward<__bf16>(p, x, weight, slope, dy, dx, d_weight, d_bias, ws, st);
+  else backward<_Float16>(p, x, weight, slope, dy, dx, d_weight, d_bias, ws, st);
   MEM_CHECK_LAUNCH(what);
   return MRL_OK;
 }

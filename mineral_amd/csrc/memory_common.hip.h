@@ -61,37 +61,48 @@ template <int N> __device__ __forceinline__ void act_fwd(int act, float (&z)[N])
     default: break;
   }
 }
-// d[e] *= act'(z[e])
-template <int N> __device__ __forceinline__ void act_bwd(int act, const float (&z)[N], float (&d)[N]) {
+// act'(z) into d
+template <int N> __device__ __forceinline__ void act_slope(int act, const float (&z)[N], float (&d)[N]) {
   switch (act) {
     case MRL_ACT_SILU:
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const float s = logistic(z[e]);
-        d[e] *= s * (1.0f + z[e] * (1.0f - s));
+        d[e] = s * (1.0f + z[e] * (1.0f - s));
       }
       break;
     case MRL_ACT_ELU:
 #pragma unroll
-      for (int e = 0; e < N; ++e) d[e] *= z[e] > 0.0f ? 1.0f : expf(z[e]);
+      for (int e = 0; e < N; ++e) d[e] = z[e] > 0.0f ? 1.0f : expf(z[e]);
       break;
     case MRL_ACT_RELU:
 #pragma unroll
-      for (int e = 0; e < N; ++e) d[e] = z[e] <= 0.0f ? 0.0f : d[e];
+      for (int e = 0; e < N; ++e) d[e] = z[e] <= 0.0f ? 0.0f : 1.0f;
       break;
     case MRL_ACT_TANH:
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const float t = tanhf(z[e]);
-        d[e] *= (1.0f - t) * (1.0f + t);
+        d[e] = (1.0f - t) * (1.0f + t);
       }
       break;
     case MRL_ACT_GELU:
 #pragma unroll
-      for (int e = 0; e < N; ++e) d[e] *= 0.5f * erfcf(z[e] * -0.70710678f) + z[e] * 0.39894228f * expf(-0.5f * z[e] * z[e]);
+      for (int e = 0; e < N; ++e) d[e] = 0.5f * erfcf(z[e] * -0.70710678f) + z[e] * 0.39894228f * expf(-0.5f * z[e] * z[e]);
       break;
-    default: break;
+    default:
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] = 1.0f;
+      break;
   }
+}
+// d[e] *= act'(z[e])
+template <int N> __device__ __forceinline__ void act_bwd(int act, const float (&z)[N], float (&d)[N]) {
+  if (act == MRL_ACT_NONE) return;
+  float s[N];
+  act_slope<N>(act, z, s);
+#pragma unroll
+  for (int e = 0; e < N; ++e) d[e] = act == MRL_ACT_RELU && s[e] == 0.0f ? 0.0f : d[e] * s[e];
 }
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }

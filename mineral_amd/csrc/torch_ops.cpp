@@ -351,15 +351,15 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w_, con
   c10::DeviceGuard guard(x.device());
   const Tensor w = w_.contiguous(), b = contiguous(b_), r = contiguous(r_);
   const auto shape = d.out_shape(x);
-  Tensor y = new_like(x, shape), z = keep && act != MRL_ACT_NONE ? new_like(x, shape) : Tensor();
-  check(mrl_linear_act(&d.p, cp(d.x), cp(w), cp(b), cp(r), mp(y), mp(z), stream_of(x)), what);
-  return {y, z};
+  Tensor y = new_like(x, shape), slope = keep && act != MRL_ACT_NONE ? new_like(x, shape) : Tensor();   // 16 or 32 bits each, like x
+  check(mrl_linear_act(&d.p, cp(d.x), cp(w), cp(b), cp(r), mp(y), mp(slope), stream_of(x)), what);
+  return {y, slope};
 }
 
 struct LinearAct : Function<LinearAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, int64_t act, int64_t needs) {
-    auto [y, z] = linear_forward(x, w, of(b), of(r), (int)act, needs & 7);
-    ctx->save_for_backward({x, w, z});
+    auto [y, slope] = linear_forward(x, w, of(b), of(r), (int)act, needs & 7);
+    ctx->save_for_backward({x, w, slope});
     ctx->saved_data["act"] = act;
     ctx->saved_data["needs"] = needs;
     return y;
