@@ -64,66 +64,98 @@ template <> struct Frag<float> {
   static __device__ __forceinline__ f32x16 mul(const F& a, const F& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
-// One operand's tile: ROWS rows (of A or B) x BK reduction indices.
-template <typename T, int LAY, int ROWS, int BK, int NTH> struct Operand {
+// One operand's tile of a step: ROWS rows (of A or B) x BK reduction indices, as lines of WIDTH elements.
+// LAY_K lines outside the matrix repeat its last one and columns beyond its edge hold what lies there: they only reach outputs that are
+// not stored.  Reduction indices beyond the end read as zero in both operands.  A step that is whole and touches nothing beyond the
+// matrix's last element (`whole`) is loaded without checks, the others element by element where a 16-byte unit is cut.
+// DIRECT: rows are whole 16-byte units on 16-byte addresses; the loads write LDS themselves (no registers, the next stage is in
+// flight during a whole step), which fixes the lines' pitch, so the 16-byte pieces of a line are permuted by its number instead to
+// spread the fragment reads over the banks.
+template <typename T, int LAY, int ROWS, int BK, int NTH, bool DIRECT> struct Operand {
   static constexpr int NP = Frag<T>::NP, E = 16 / (int)sizeof(T);
-  // LDS image: [ROWS][BK] or [BK][ROWS] 16-bit values, row pitches that spread the fragment reads over the banks
+  static_assert(!DIRECT || NP == 1, "fp32 is split on its way to LDS");
   static constexpr int LINES = LAY == LAY_K ? ROWS : BK, WIDTH = LAY == LAY_K ? BK : ROWS;
-  static constexpr int PITCH = WIDTH * 2 + (LAY == LAY_K ? 16 : 64);
+  static constexpr int PITCH = WIDTH * 2 + (DIRECT ? 0 : LAY == LAY_K ? 16 : 64);
   static constexpr int PLANE = LINES * PITCH, BYTES = PLANE * NP;
   static constexpr int UPL = WIDTH / E, UNITS = LINES * UPL, U = (UNITS + NTH - 1) / NTH;
-  u32x4 r[U];
-  const T* p[U];          // this thread's units of the next tile
-  int64_t left[U];        // elements up to the end of the line; none where the line is outside
+  static_assert(!DIRECT || (UNITS % NTH == 0 && (LAY == LAY_R || UPL == 4 || UPL == 8)), "whole waves, known line widths");
+  u32x4 r[DIRECT ? 1 : U];
+  const T* p[U];          // this thread's units of the next step
+  int left[U];            // LAY_R: columns from the unit to the matrix's edge
+  bool edge;              // LAY_R: the tile has units that are cut by the edge
 
-  // row0: first row of the tile; lines beyond `rows` (LAY_K) or beyond r1 (LAY_R) read as zero
-  __device__ __forceinline__ void init(const void* base, int64_t ld, int64_t row0, int64_t rows, int64_t r0, int64_t r1, int tid) {
+  // which 16-byte piece of line `line` lies at piece `at`
+  static __device__ __forceinline__ int piece(int line, int at) {
+    if constexpr (!DIRECT) return at;
+    else if constexpr (LAY == LAY_K) return at ^ ((line >> (UPL == 8 ? 1 : 2)) & (UPL - 1));   // 16 neighbouring lines cover the banks
+    else return at ^ ((line & 3) << 1 & (UPL - 1));
+  }
+  __device__ __forceinline__ void init(const void* base, int64_t ld, int64_t row0, int64_t rows, int64_t r0, int tid) {
+    edge = LAY == LAY_R && rows % E != 0 && row0 + WIDTH > rows;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = tid + NTH * i, line = u / UPL, c = (u % UPL) * E;
+      const int u = tid + NTH * i, line = u / UPL, c = piece(line, u % UPL) * E;
       if constexpr (LAY == LAY_K) {
-        p[i] = static_cast<const T*>(base) + (row0 + line) * ld + r0 + c;
-        left[i] = (u < UNITS && row0 + line < rows) ? r1 - r0 - c : 0;
+        p[i] = static_cast<const T*>(base) + min(row0 + line, rows - 1) * ld + r0 + c;
       } else {
-        p[i] = static_cast<const T*>(base) + (r0 + line) * ld + row0 + c;
-        left[i] = u < UNITS ? rows - row0 - c : 0;
+        const bool in = row0 + c < rows;
+        p[i] = static_cast<const T*>(base) + (r0 + line) * ld + (in ? row0 + c : 0);
+        left[i] = (int)min<int64_t>(E, in ? rows - row0 - c : rows);
       }
     }
   }
-  __device__ __forceinline__ void load(int64_t ld, int64_t r0, int64_t r1, int tid) {
+  // the unit of a step that is not whole
+  __device__ __forceinline__ u32x4 cut(int i, int64_t left_r, int tid) const {
+    const int u = tid + NTH * i, line = u / UPL;
+    if constexpr (LAY == LAY_K) return load_unit(p[i], left_r - piece(line, u % UPL) * E);
+    else return load_unit(p[i], line < left_r ? left[i] : 0);
+  }
+  // A whole step.  wave0: the first thread of this wave, as a scalar.
+  __device__ __forceinline__ void load(int64_t ld, char* tile, int wave0) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int line = (tid + NTH * i) / UPL;
-      if constexpr (LAY == LAY_K) {
-        r[i] = load_unit(p[i], left[i]);
-        p[i] += BK;
-        left[i] -= BK;
-      } else {
-        r[i] = load_unit(p[i], r0 + line < r1 ? left[i] : 0);
-        p[i] += BK * ld;
-      }
+      if constexpr (DIRECT) {
+        // As asm without outputs: for the builtin the compiler waits for every such load before the next read of LDS, which would
+        // undo the prefetch; here the barrier of the main loop counts them (its own waits only become stricter by them).  The
+        // hardware writes lane l's 16 bytes at m0 + 16 l.
+        const unsigned at = (unsigned)(uintptr_t)(tile + (i * NTH + wave0) * 16);   // the low half of an LDS address is its offset
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p[i]), "s"(at) : "memory", "m0");
+      } else __builtin_memcpy(&r[i], p[i], 16);
+      p[i] += LAY == LAY_K ? BK : BK * ld;
+    }
+  }
+  // Any other step: left_r reduction indices from its first to the end.
+  __device__ __forceinline__ void load_cut(int64_t ld, int64_t left_r, char* tile, int tid) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const u32x4 w = cut(i, left_r, tid);
+      if constexpr (DIRECT) *reinterpret_cast<u32x4*>(tile + (i * NTH + tid) * 16) = w;
+      else r[i] = w;
+      p[i] += LAY == LAY_K ? BK : BK * ld;
     }
   }
   __device__ __forceinline__ void store(char* tile, int tid) const {
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = tid + NTH * i;
-      if (UNITS % NTH == 0 || u < UNITS) {
-        char* q = tile + (u / UPL) * PITCH + (u % UPL) * E * 2;
-        if constexpr (NP == 1) *reinterpret_cast<u32x4*>(q) = r[i];
-        else {
-          u32x2 h, m, l;
+      for (int i = 0; i < U; ++i) {
+        const int u = tid + NTH * i;
+        if (UNITS % NTH == 0 || u < UNITS) {
+          char* q = tile + (u / UPL) * PITCH + (u % UPL) * E * 2;
+          if constexpr (NP == 1) *reinterpret_cast<u32x4*>(q) = r[i];
+          else {
+            u32x2 h, m, l;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x0 = __uint_as_float(r[i][2 * e]), x1 = __uint_as_float(r[i][2 * e + 1]);
-            h[e] = pack_bf16(x0, x1);
-            const float a0 = x0 - half_lo(h[e]), a1 = x1 - half_hi(h[e]);
-            m[e] = pack_bf16(a0, a1);
-            l[e] = pack_bf16(a0 - half_lo(m[e]), a1 - half_hi(m[e]));
+            for (int e = 0; e < 2; ++e) {
+              const float x0 = __uint_as_float(r[i][2 * e]), x1 = __uint_as_float(r[i][2 * e + 1]);
+              h[e] = pack_bf16(x0, x1);
+              const float a0 = x0 - half_lo(h[e]), a1 = x1 - half_hi(h[e]);
+              m[e] = pack_bf16(a0, a1);
+              l[e] = pack_bf16(a0 - half_lo(m[e]), a1 - half_hi(m[e]));
+            }
+            *reinterpret_cast<u32x2*>(q) = h;
+            *reinterpret_cast<u32x2*>(q + PLANE) = m;
+            *reinterpret_cast<u32x2*>(q + 2 * PLANE) = l;
           }
-          *reinterpret_cast<u32x2*>(q) = h;
-          *reinterpret_cast<u32x2*>(q + PLANE) = m;
-          *reinterpret_cast<u32x2*>(q + 2 * PLANE) = l;
         }
       }
     }
@@ -132,11 +164,13 @@ template <typename T, int LAY, int ROWS, int BK, int NTH> struct Operand {
   static __device__ __forceinline__ typename Frag<T>::F frag(const char* tile, int plane, int row, int ks, int lane) {
     const char* t = tile + plane * PLANE;
     if constexpr (LAY == LAY_K) {
-      return __builtin_bit_cast(typename Frag<T>::F, *reinterpret_cast<const u32x4*>(t + (row + (lane & 31)) * PITCH + (16 * ks + 8 * (lane >> 5)) * 2));
+      const int line = row + (lane & 31);
+      return __builtin_bit_cast(typename Frag<T>::F, *reinterpret_cast<const u32x4*>(t + line * PITCH + piece(line, 2 * ks + (lane >> 5)) * 16));
     } else {
       // a 16-lane group names four lines of 16 columns, 8 bytes a lane, and every lane gets its column of them
       typedef s16x4 __attribute__((address_space(3))) * lds_p;
-      const char* a = t + (16 * ks + 8 * (lane >> 5) + ((lane >> 2) & 3)) * PITCH + (row + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+      const int line = 16 * ks + 8 * (lane >> 5) + ((lane >> 2) & 3), col = row + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const char* a = t + line * PITCH + piece(line, col >> 3) * 16 + (col & 7) * 2;   // line + 4 has the same permutation
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 4 * PITCH));
       return __builtin_bit_cast(typename Frag<T>::F, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -197,7 +231,8 @@ template <typename S> __device__ __forceinline__ void store_slopes(S* p, int lef
     u32x4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = pack_slope(x[2 * e]) | pack_slope(x[2 * e + 1]) << 16;
-    if (left >= 8) __builtin_memcpy(p, &w, 16);
+    typedef u32x4 __attribute__((aligned(2))) unit;
+    if (left >= 8) __builtin_nontemporal_store(w, reinterpret_cast<unit*>(p));
     else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -206,32 +241,166 @@ template <typename S> __device__ __forceinline__ void store_slopes(S* p, int lef
   }
 }
 
-// WM x WN waves over the tile, WK waves over the reduction inside a step
-template <typename T, int BM, int BN, int BK, int WM, int WN, int WK, int LA, int LB, int NBUF>
+// Consecutive blocks go to the 8 XCDs in turn: each XCD gets a run of neighbouring tiles, so that its L2 holds what they share.
+struct Tile { int split, n0; int64_t m0, r0, r1; bool none; };
+template <int BM, int BN> __device__ __forceinline__ Tile tile_of(const MmP& p) {
+  Tile t;
+  const int tiles = p.m_tiles * p.n_tiles, per = gridDim.x / 8;
+  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3), tile = id % tiles;
+  t.none = id >= p.blocks;                                // the grid is padded to a multiple of 8
+  t.split = id / tiles;
+  t.m0 = (int64_t)(tile / p.n_tiles) * BM;
+  t.n0 = (tile % p.n_tiles) * BN;
+  t.r0 = t.split * p.r_split;
+  t.r1 = min(p.R, t.r0 + p.r_split);
+  return t;
+}
+
+// Eight values in units that are not read again soon: past the L2, which holds what the tiles share (W and the rows of x)
+template <typename T> __device__ __forceinline__ void stream8(T* p, const T (&x)[8]) {
+  typedef u32x4 __attribute__((aligned(2))) unit;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    u32x4 w;
+    __builtin_memcpy(&w, x + i * 16 / sizeof(T), 16);
+    __builtin_nontemporal_store(w, reinterpret_cast<unit*>(p) + i);
+  }
+}
+template <typename T> __device__ __forceinline__ void stream_row(T* p, int left, const float (&x)[8]) {
+  if (left >= 8) {
+    T v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (T)x[e];
+    stream8(p, v);
+  } else store_row<T, 8>(p, left, x);
+}
+
+template <typename T, int ACT> __device__ __forceinline__ void finish8(const MmP& p, int64_t at, int left, float (&v)[8], const float (&bias)[8], const T (&res)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += bias[e];
+  if (ACT != MRL_ACT_NONE && p.slope) {
+    typedef typename SlopeOf<T>::S S;
+    float d[8];
+    act_slope<8>(ACT, v, d);
+    store_slopes<S>(static_cast<S*>(p.slope) + at, left, d);
+  }
+  act_fwd<8>(ACT, v);
+  if (p.residual) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += (float)res[e];
+  }
+  stream_row<T>(static_cast<T*>(p.y) + at, left, v);
+}
+
+// The epilogue of a wave's TM x TN accumulators, by itself: 32 rows at a time go through its own piece of LDS and leave in units of 8
+// columns, whole cache lines of a row.  The residuals are on their way since the last step.
+template <typename T, int TM, int TN, bool PLAIN> struct WaveEpilogue {
+  static constexpr int W = TN * 32, EP = W + 4, BYTES = 32 * EP * 4, UPR = W / 8, UNITS = 32 * UPR / 64;
+  typedef T row8[8];
+  static constexpr int AHEAD = TM < 2 ? TM : 2;             // 32-row pieces of the residual in registers
+  typedef row8 Residual[AHEAD][UNITS];
+  static __device__ __forceinline__ void fetch(const MmP& p, int64_t m, int n, int lane, row8 (&res)[UNITS]) {
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const int u = lane + 64 * i, c = n + (u % UPR) * 8, left = p.N - c;
+      const int64_t row = m + u / UPR;
+      if (row < p.M && left > 0) {
+        const T* q = static_cast<const T*>(p.residual) + row * p.N + c;
+        if (left >= 8) {
+          typedef u32x4 __attribute__((aligned(2))) unit;
+#pragma unroll
+          for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+            const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const unit*>(q) + h);
+            __builtin_memcpy(res[i] + h * 16 / sizeof(T), &w, 16);
+          }
+        }
+        else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) res[i][e] = e < left ? q[e] : (T)0.0f;
+        }
+      }
+    }
+  }
+  // the first pieces of the residual: issued before the wave's last products
+  static __device__ __forceinline__ void fetch_first(const MmP& p, int64_t m, int n, int lane, Residual& res) {
+    if (PLAIN || !p.residual) return;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(p, m + 32 * i, n, lane, res[i]);
+  }
+  template <int ACT>
+  static __device__ __forceinline__ void run_act(const MmP& p, const Tile& t, float* lds, const f32x16 (&acc)[TN][TM], int64_t m, int n, int lane, Residual& res) {
+    float bias[8];
+    const int c = n + (lane % UPR) * 8, left = p.N - c;     // 64 is a multiple of UPR: a lane's columns stay
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bias[e] = 0.0f;
+    if (!PLAIN && p.bias && left > 0) load_row<T, 8>(static_cast<const T*>(p.bias) + c, left, bias);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(lds + (lane & 31) * EP + j * 32 + 8 * q + 4 * (lane >> 5)) =
+              f32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+      __builtin_amdgcn_wave_barrier();                      // one wave: its LDS operations stay in order
+#pragma unroll
+      for (int k = 0; k < UNITS; ++k) {
+        const int u = lane + 64 * k;
+        const int64_t row = m + 32 * i + u / UPR;
+        float v[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 s = *reinterpret_cast<const f32x4*>(lds + (u / UPR) * EP + (u % UPR) * 8 + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * h + e] = s[e];
+        }
+        if (row < p.M && left > 0) {
+          const int64_t at = row * p.N + c;
+          if (PLAIN && p.slab) store_row<float, 8>(p.slab + (int64_t)t.split * p.M * p.N + at, left, v);
+          else if (PLAIN) store_row<T, 8>(static_cast<T*>(p.y) + at, left, v);
+          else finish8<T, ACT>(p, at, left, v, bias, res[i % AHEAD][k]);
+        }
+      }
+      if (!PLAIN && p.residual && i + AHEAD < TM) fetch(p, m + 32 * (i + AHEAD), n, lane, res[i % AHEAD]);
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  static __device__ __forceinline__ void run(const MmP& p, const Tile& t, float* lds, const f32x16 (&acc)[TN][TM], int64_t m, int n, int lane, Residual& res) {
+    if constexpr (PLAIN) run_act<MRL_ACT_NONE>(p, t, lds, acc, m, n, lane, res);
+    else switch (p.act) {                                   // one straight path per activation
+      case MRL_ACT_SILU: run_act<MRL_ACT_SILU>(p, t, lds, acc, m, n, lane, res); break;
+      case MRL_ACT_ELU: run_act<MRL_ACT_ELU>(p, t, lds, acc, m, n, lane, res); break;
+      case MRL_ACT_RELU: run_act<MRL_ACT_RELU>(p, t, lds, acc, m, n, lane, res); break;
+      case MRL_ACT_TANH: run_act<MRL_ACT_TANH>(p, t, lds, acc, m, n, lane, res); break;
+      case MRL_ACT_GELU: run_act<MRL_ACT_GELU>(p, t, lds, acc, m, n, lane, res); break;
+      default: run_act<MRL_ACT_NONE>(p, t, lds, acc, m, n, lane, res); break;
+    }
+  }
+};
+
+// WM x WN waves over the tile, WK waves over the reduction inside a step; NST stages in LDS, NST - 1 steps of loads in flight (DIRECT),
+// or loads through registers one step ahead with NST 1 or 2 stages.
+template <typename T, int BM, int BN, int BK, int WM, int WN, int WK, int LA, int LB, int NST, bool DIRECT>
 __global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
   constexpr int NTH = WM * WN * WK * 64, TM = BM / WM / 32, TN = BN / WN / 32, KS = BK / 16 / WK, NP = Frag<T>::NP;
-  typedef Operand<T, LA, BM, BK, NTH> OA;
-  typedef Operand<T, LB, BN, BK, NTH> OB;
+  constexpr bool PLAIN = LB == LAY_R;                      // a gradient: no epilogue but the store
+  typedef Operand<T, LA, BM, BK, NTH, DIRECT> OA;
+  typedef Operand<T, LB, BN, BK, NTH, DIRECT> OB;
   typedef typename Frag<T>::F F;
-  constexpr int STAGE = OA::BYTES + OB::BYTES, EP = BN + 4, EBYTES = WK * BM * EP * 4;
-  constexpr int LDS = NBUF * STAGE > EBYTES ? NBUF * STAGE : EBYTES;
+  typedef WaveEpilogue<T, TM, TN, PLAIN> WE;
+  static_assert(WK == 1 || (TM == 1 && TN == 1), "shared reductions: one tile a wave");
+  constexpr int STAGE = OA::BYTES + OB::BYTES, EBYTES = WE::BYTES * WM * WN * WK;
+  constexpr int LDS = NST * STAGE > EBYTES ? NST * STAGE : EBYTES;
   __shared__ __attribute__((aligned(16))) char lds[LDS];
-  // consecutive blocks go to the 8 XCDs in turn: each XCD gets a run of neighbouring tiles, so that its L2 holds what they share
-  const int tiles = p.m_tiles * p.n_tiles;
-  const int per = (gridDim.x + 7) / 8;
-  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  const int split = id / tiles, tile = id % tiles;
-  if (id >= p.blocks) return;                            // the grid is padded to a multiple of 8
-  const int64_t m0 = (int64_t)(tile / p.n_tiles) * BM;
-  const int n0 = (tile % p.n_tiles) * BN;
+  const Tile t = tile_of<BM, BN>(p);
+  if (t.none) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wk = wave % WK, wn = wave / WK % WN, wm = wave / (WK * WN);
-  const int64_t r0 = split * p.r_split, r1 = min(p.R, r0 + p.r_split);
 
   OA oa;
   OB ob;
-  oa.init(p.a, p.lda, m0, p.M, r0, r1, tid);
-  ob.init(p.b, p.ldb, n0, p.N, r0, r1, tid);
+  oa.init(p.a, p.lda, t.m0, p.M, t.r0, tid);
+  ob.init(p.b, p.ldb, t.n0, p.N, t.r0, tid);
   f32x16 acc[TN][TM];
 #pragma unroll
   for (int j = 0; j < TN; ++j)
@@ -240,7 +409,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.0f;
 
-  const int steps = (int)((r1 - r0 + BK - 1) / BK);
+  const int steps = (int)((t.r1 - t.r0 + BK - 1) / BK);
   auto multiply = [&](const char* st) {
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
@@ -268,96 +437,83 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
         }
     }
   };
-  if (steps > 0) {
-    oa.load(p.lda, r0, r1, tid);
-    ob.load(p.ldb, r0, r1, tid);
-  }
-  if constexpr (NBUF == 2) {
+  // Steps that are loaded without checks: those of BK indices; beside a cut edge, whose units reach up to 7 elements, so at most as
+  // many lines, too far, only those that far from the matrix's end.
+  const int64_t span = t.r1 - t.r0, room = oa.edge || ob.edge ? min(span, p.R - t.r0 - 8) : span;
+  const int whole = (int)(room > 0 ? room / BK : 0), wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);
+  auto load = [&](int s, char* st) {
+    if (s < whole) {
+      oa.load(p.lda, st, wave0);
+      ob.load(p.ldb, st + OA::BYTES, wave0);
+    } else {
+      oa.load_cut(p.lda, span - (int64_t)s * BK, st, tid);
+      ob.load_cut(p.ldb, span - (int64_t)s * BK, st + OA::BYTES, tid);
+    }
+  };
+  const int64_t wave_m = t.m0 + wm * TM * 32;
+  const int wave_n = t.n0 + wn * TN * 32;
+  typename WE::Residual res;
+  auto store = [&](char* st) {
+    oa.store(st, tid);
+    ob.store(st + OA::BYTES, tid);
+  };
+  if constexpr (DIRECT) {
+    constexpr int L = OA::U + OB::U;                       // loads of a step, each counted once by vmcnt
+    static_assert((NST - 2) * L < 64, "vmcnt");
+#pragma unroll
+    for (int s = 0; s < NST - 1; ++s)
+      if (s < steps) load(s, lds + s * STAGE);
+    int at = 0;
+    for (int s = 0; s < steps; ++s) {
+      // This wave's share of stage s has landed when no more than the later steps' loads are outstanding; the last steps, which
+      // have fewer behind them (and maybe a cut one, loaded through registers), wait for everything.  Behind the barrier every
+      // wave's share has landed and every wave has left the stage that is filled next.  (__syncthreads would wait for all loads.)
+      if (s + NST - 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NST - 2) * L) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + NST - 1 < steps) load(s + NST - 1, lds + (at == 0 ? NST - 1 : at - 1) * STAGE);
+      if (s + 1 == steps) WE::fetch_first(p, wave_m, wave_n, lane, res);
+      multiply(lds + at * STAGE);
+      at = at + 1 == NST ? 0 : at + 1;
+    }
+  } else if constexpr (NST == 2) {
     if (steps > 0) {
-      oa.store(lds, tid);
-      ob.store(lds + OA::BYTES, tid);
+      load(0, lds);
+      store(lds);
     }
     for (int s = 0; s < steps; ++s) {
-      if (s + 1 < steps) {
-        oa.load(p.lda, r0 + (int64_t)(s + 1) * BK, r1, tid);
-        ob.load(p.ldb, r0 + (int64_t)(s + 1) * BK, r1, tid);
-      }
-      __syncthreads();                       // stage s is written, and every wave has left the one that s + 1 goes to
+      if (s + 1 < steps) load(s + 1, lds);
+      else WE::fetch_first(p, wave_m, wave_n, lane, res);
+      __syncthreads();                                     // stage s is written, and every wave has left the one that s + 1 goes to
       multiply(lds + (s & 1) * STAGE);
-      if (s + 1 < steps) {
-        char* next = lds + ((s + 1) & 1) * STAGE;
-        oa.store(next, tid);
-        ob.store(next + OA::BYTES, tid);
-      }
+      if (s + 1 < steps) store(lds + ((s + 1) & 1) * STAGE);
     }
   } else {
+    if (steps > 0) load(0, lds);
     for (int s = 0; s < steps; ++s) {
-      oa.store(lds, tid);
-      ob.store(lds + OA::BYTES, tid);
-      if (s + 1 < steps) {
-        oa.load(p.lda, r0 + (int64_t)(s + 1) * BK, r1, tid);
-        ob.load(p.ldb, r0 + (int64_t)(s + 1) * BK, r1, tid);
-      }
+      store(lds);
+      if (s + 1 < steps) load(s + 1, lds);
+      else WE::fetch_first(p, wave_m, wave_n, lane, res);
       __syncthreads();
       multiply(lds);
       __syncthreads();
     }
   }
-
-  // ---- epilogue: rows of the tile from LDS
-  __syncthreads();
-  float* ep = reinterpret_cast<float*>(lds);
+  if (steps == 0) WE::fetch_first(p, wave_m, wave_n, lane, res);
+  __syncthreads();                                         // the stages are free
+  float* ep = reinterpret_cast<float*>(lds) + wave * (WE::BYTES / 4);
+  if constexpr (WK > 1) {                                  // the waves' shares, added in order by the first
+    if (wk > 0) {
 #pragma unroll
-  for (int j = 0; j < TN; ++j)
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int row = wk * BM + (wm * TM + i) * 32 + (lane & 31), col = (wn * TN + j) * 32 + 8 * q + 4 * (lane >> 5);
-        *reinterpret_cast<f32x4*>(ep + row * EP + col) = f32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-      }
-  __syncthreads();
-  constexpr int UPR = BN / 8;
-  for (int u = tid; u < BM * UPR; u += NTH) {
-    const int row = u / UPR, c = (u % UPR) * 8;
-    const int64_t m = m0 + row;
-    const int left = p.N - n0 - c;
-    if (m >= p.M || left <= 0) continue;
-    float v[8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 s = *reinterpret_cast<const f32x4*>(ep + row * EP + c + 4 * h);
-#pragma unroll
-      for (int k = 1; k < WK; ++k) s += *reinterpret_cast<const f32x4*>(ep + (k * BM + row) * EP + c + 4 * h);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * h + e] = s[e];
+      for (int e = 0; e < 16; ++e) ep[e * 64 + lane] = acc[0][0][e];
     }
-    const int64_t at = m * p.N + n0 + c;
-    if (p.slab) {
-      store_row<float, 8>(p.slab + (int64_t)split * p.M * p.N + at, left, v);
-      continue;
-    }
-    if (p.bias) {
-      float b[8];
-      load_row<T, 8>(static_cast<const T*>(p.bias) + n0 + c, left, b);
+    __syncthreads();
+    if (wk > 0) return;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += b[e];
-    }
-    if (p.slope) {
-      typedef typename SlopeOf<T>::S S;
-      float d[8];
-      act_slope<8>(p.act, v, d);
-      store_slopes<S>(static_cast<S*>(p.slope) + at, left, d);
-    }
-    act_fwd<8>(p.act, v);
-    if (p.residual) {
-      float b[8];
-      load_row<T, 8>(static_cast<const T*>(p.residual) + at, left, b);
+    for (int k = 1; k < WK; ++k)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += b[e];
-    }
-    store_row<T, 8>(static_cast<T*>(p.y) + at, left, v);
+      for (int e = 0; e < 16; ++e) acc[0][0][e] += ep[k * (WE::BYTES / 4) + e * 64 + lane];
   }
+  WE::run(p, t, ep, acc, wave_m, wave_n, lane, res);
 }
 
 // dz = dy slope, and the sums of its columns over this block's rows -> part [blocks in y][N].  32 units of 8 columns x 8 rows a block.
@@ -372,17 +528,26 @@ __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* _
   for (int e = 0; e < 8; ++e) s[e] = 0.0f;
   if (left > 0) {
     const int64_t m1 = min(M, ((int64_t)blockIdx.y + 1) * rows);
-    for (int64_t m = (int64_t)blockIdx.y * rows + rl; m < m1; m += 8) {
-      float d[8], g[8];
-      load_row<T, 8>(dy + m * N + c, left, d);
-      if (slope) {
-        load_slopes(slope + m * N + c, left, g);
+    constexpr int U = sizeof(T) == 2 ? 4 : 2;               // rows in flight
+    for (int64_t m = (int64_t)blockIdx.y * rows + rl; m < m1; m += 8 * U) {
+      float d[U][8], g[U][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = g[e] == 0.0f ? 0.0f : d[e] * g[e];
-        store_row<T, 8>(dz + m * N + c, left, d);
-      }
+      for (int u = 0; u < U; ++u)
+        if (m + 8 * u < m1) {
+          load_row<T, 8>(dy + (m + 8 * u) * N + c, left, d[u]);
+          if (slope) load_slopes(slope + (m + 8 * u) * N + c, left, g[u]);
+        }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += d[e];
+      for (int u = 0; u < U; ++u)
+        if (m + 8 * u < m1) {
+          if (slope) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[u][e] = g[u][e] == 0.0f ? 0.0f : d[u][e] * g[u][e];
+            store_row<T, 8>(dz + (m + 8 * u) * N + c, left, d[u]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[e] += d[u][e];
+        }
     }
   }
   if (!part) return;
@@ -453,20 +618,41 @@ int check(const mrl_linear* p, const char* what) {
 
 // Tile edge: 128 where its tiles fill the card, otherwise smaller ones, whose reduction is shared by the block's waves at 32.
 int edge_of(int64_t m, int64_t n) {
+  if (cdiv(m, 256) * cdiv(n, 256) >= 200 && n >= 192) return 256;
   if (cdiv(m, 128) * cdiv(n, 128) >= 256) return 128;
   if (cdiv(m, 64) * cdiv(n, 64) >= 256) return 64;
   return 32;
 }
 
+// rows on 16-byte addresses, for the loads that write LDS themselves
+bool direct_ok(const void* base, int64_t ld, int es) { return ((uintptr_t)base & 15) == 0 && ld * es % 16 == 0; }
+
 template <typename T, int LA, int LB> void multiply(MmP& a, int edge, int splits, hipStream_t st) {
+  const bool direct = sizeof(T) == 2 && direct_ok(a.a, a.lda, 2) && direct_ok(a.b, a.ldb, 2);
+  if (edge == 256 && (!direct || LB == LAY_K)) edge = 128;
   a.m_tiles = (int)cdiv(a.M, edge);
   a.n_tiles = (int)cdiv(a.N, edge);
   a.blocks = a.m_tiles * a.n_tiles * splits;
   const dim3 grid((unsigned)(cdiv(a.blocks, 8) * 8));
-  constexpr bool F32 = sizeof(T) == 4;
-  if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, F32 ? 32 : 64, 2, 2, 1, LA, LB, F32 ? 1 : 2>), grid, dim3(256), 0, st, a);
-  else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, F32 ? 32 : 64, 2, 2, 1, LA, LB, F32 ? 1 : 2>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, F32 ? 1 : 2>), grid, dim3(256), 0, st, a);
+  if constexpr (sizeof(T) == 4) {
+    if (edge >= 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
+    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
+  } else if (direct) {
+    if constexpr (LB == LAY_R) {
+      if (edge == 256) {
+        hipLaunchKernelGGL((mm_kernel<T, 256, 256, 32, 2, 4, 1, LA, LB, 4, true>), grid, dim3(512), 0, st, a);
+        return;
+      }
+    }
+    if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 4, true>), grid, dim3(256), 0, st, a);
+    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 64, 2, 2, 1, LA, LB, 4, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 8, true>), grid, dim3(256), 0, st, a);
+  } else {
+    if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 64, 2, 2, 1, LA, LB, 2, false>), grid, dim3(256), 0, st, a);
+    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 64, 2, 2, 1, LA, LB, 2, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 2, false>), grid, dim3(256), 0, st, a);
+  }
 }
 
 struct Plan { int edge_x, edge_w, splits; int64_t r_split; int rows, parts; int64_t dz, part, slab, total; };
@@ -476,9 +662,9 @@ Plan plan_of(const mrl_linear* p) {
   const int64_t es = p->dtype == MRL_F32 ? 4 : 2;
   r.edge_x = edge_of(p->rows, p->inputs);
   // dW: 128 x 128 tiles where both widths have them; rows split so that about 512 blocks run, in whole steps of 64
-  r.edge_w = std::min(p->inputs, p->outputs) >= 96 ? 128 : std::min(p->inputs, p->outputs) >= 48 ? 64 : 32;
+  r.edge_w = std::min(p->inputs, p->outputs) >= 192 && std::max(p->inputs, p->outputs) >= 512 && p->rows >= 4096 ? 256 : std::min(p->inputs, p->outputs) >= 96 ? 128 : std::min(p->inputs, p->outputs) >= 48 ? 64 : 32;
   const int64_t tiles = std::max<int64_t>(1, cdiv(p->outputs, r.edge_w) * cdiv(p->inputs, r.edge_w));
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(512, tiles), cdiv(p->rows, 256)));
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(r.edge_w == 256 ? 256 : 512, tiles), cdiv(p->rows, 256)));
   r.r_split = std::max<int64_t>(64, cdiv(cdiv(p->rows, splits), 64) * 64);
   r.splits = (int)std::max<int64_t>(1, cdiv(p->rows, r.r_split));
   // dz: blocks of 256 columns, about 2048 of them

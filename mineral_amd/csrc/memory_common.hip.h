@@ -34,8 +34,16 @@ __device__ __forceinline__ float half_lo(unsigned pk) { return __uint_as_float(p
 __device__ __forceinline__ float half_hi(unsigned pk) { return __uint_as_float(pk & 0xffff0000u); }
 
 // Activations and their derivatives at z, in fp32.  `act` is uniform over the launch.  The logistic function uses the hardware's
-// exp2 and reciprocal (one spacing each); where a difference cancels near zero (ELU, tanh, erf) the library's functions do.
+// exp2 and reciprocal (one spacing each); where a difference cancels near zero (ELU, erf) the library's functions do.
 __device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+// tanh from its series up to 1/4 (the first term left out is below 1e-8 of it) and from exp2 beyond, where the difference from one
+// loses at most two bits
+__device__ __forceinline__ float tanh_of(float z) {
+  const float q = z * z, a = __builtin_fabsf(z);
+  const float low = z * __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, __builtin_fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  const float high = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * 2.88539008f));
+  return a < 0.25f ? low : __builtin_copysignf(high, z);
+}
 template <int N> __device__ __forceinline__ void act_fwd(int act, float (&z)[N]) {
   switch (act) {
     case MRL_ACT_SILU:
@@ -52,7 +60,7 @@ template <int N> __device__ __forceinline__ void act_fwd(int act, float (&z)[N])
       break;
     case MRL_ACT_TANH:
 #pragma unroll
-      for (int e = 0; e < N; ++e) z[e] = tanhf(z[e]);
+      for (int e = 0; e < N; ++e) z[e] = tanh_of(z[e]);
       break;
     case MRL_ACT_GELU:
 #pragma unroll
@@ -82,7 +90,7 @@ template <int N> __device__ __forceinline__ void act_slope(int act, const float 
     case MRL_ACT_TANH:
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float t = tanhf(z[e]);
+        const float t = tanh_of(z[e]);
         d[e] = (1.0f - t) * (1.0f + t);
       }
       break;
