@@ -12,15 +12,16 @@
 // (or 32) value columns and all rows of S in MFMA accumulators for the whole segment.  The products are arranged so that every
 // intermediate is the next product's operand where it lies: with 16x16x32 MFMAs a lane's accumulators of two stacked 16-row tiles
 // are rows {4g..4g+3, 16+4g..16+4g+3} of its column (g = lane / 16), and any order of the reduction index serves as long as both
-// operands share it, so S and P^T go from accumulators to operands without LDS; row-major operands are read from LDS as two
-// 8-byte pieces in that order, token-major ones through the transposing LDS read, whose 16-lane groups return exactly four rows of
+// operands share it, so S and P^T go from accumulators to operands without LDS; row-major operands lie in LDS in that order and are
+// read in 16-byte pieces, token-major ones through the transposing LDS read, whose 16-lane groups return exactly four rows of
 // a column.  Only q, k, v pass through LDS (registers hold the next chunk meanwhile).  The scores are computed by every wave:
 // matrix work is not what bounds the kernel, an exchange through LDS with its barriers would.
 //
 // Precision: everything accumulates in fp32.  16-bit inputs multiply as they are (fp16 as two exact bf16 terms where the partner
 // is an fp32 intermediate, whose range fp16 lacks); an fp32 intermediate enters a product as two bf16 terms (P, S: 2^-17 relative,
-// below the rounding of the 16-bit outputs) or three (the weighted v of the state, which stays fp32: 2^-24).  fp32 inputs use the
-// fp32 MFMA throughout.
+// below the rounding of the 16-bit outputs) or three (the weighted v of the state, which stays fp32: 2^-24).  fp32 inputs become
+// three exact bf16 terms on their way to LDS and multiply in six products, like every intermediate beside them: 2^-23, and 2.7 times
+// the rate of the fp32 MFMA.
 //
 // Masked tokens: weights are applied by selection, and a chunk that holds an infinity or NaN is walked token by token (the same
 // code with chunks of one), so that a zero weight never meets one: nothing of a later token or an earlier episode leaks.
@@ -128,23 +129,36 @@ __device__ __forceinline__ void mma(f32x4& c, const Planes2& a, const Planes3& b
   c = mfma_bf(a.p[0], b.p[1], c);
   c = mfma_bf(a.p[0], b.p[0], c);
 }
-__device__ __forceinline__ void mma(f32x4& c, const f32x8& a, const f32x8& b) {       // step e reduces over rows {4g + e} of a 16-row half
-#pragma unroll
-  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+__device__ __forceinline__ void mma(f32x4& c, const Planes3& a, const Planes3& b) {   // without the three terms below 2^-23
+  c = mfma_bf(a.p[2], b.p[0], c);
+  c = mfma_bf(a.p[0], b.p[2], c);
+  c = mfma_bf(a.p[1], b.p[1], c);
+  c = mfma_bf(a.p[1], b.p[0], c);
+  c = mfma_bf(a.p[0], b.p[1], c);
+  c = mfma_bf(a.p[0], b.p[0], c);
 }
 
 template <typename T> struct El;
 template <> struct El<float> {
-  static constexpr int C = 32;
-  typedef f32x8 Raw; typedef f32x8 In; typedef f32x8 De; typedef f32x8 Wt;
+  static constexpr int C = 32, PLANES = 3;
+  typedef Planes3 Raw; typedef Planes3 In; typedef Planes3 De; typedef Planes3 Wt;
   static __device__ __forceinline__ In in(const Raw& r) { return r; }
-  static __device__ __forceinline__ De de(const f32x8& x) { return x; }
-  static __device__ __forceinline__ Wt wt(const f32x8& x) { return x; }
-  static __device__ __forceinline__ f32x8 wide(const Raw& r) { return r; }
+  static __device__ __forceinline__ De de(const f32x8& x) { return split3(x); }
+  static __device__ __forceinline__ Wt wt(const f32x8& x) { return split3(x); }
+  static __device__ __forceinline__ f32x8 wide(const Raw& r) {               // the exact sum again
+    f32x8 x;
+    const u32x4 h = __builtin_bit_cast(u32x4, r.p[0]), m = __builtin_bit_cast(u32x4, r.p[1]), l = __builtin_bit_cast(u32x4, r.p[2]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[2 * e] = half_lo(h[e]) + (half_lo(m[e]) + half_lo(l[e]));
+      x[2 * e + 1] = half_hi(h[e]) + (half_hi(m[e]) + half_hi(l[e]));
+    }
+    return x;
+  }
   static __device__ __forceinline__ void score(f32x4& c, const Raw& a, const Raw& b) { mma(c, a, b); }
 };
 template <> struct El<__bf16> {
-  static constexpr int C = 64;
+  static constexpr int C = 64, PLANES = 1;
   typedef bf16x8 Raw; typedef Planes1 In; typedef Planes2 De; typedef Planes3 Wt;
   static __device__ __forceinline__ In in(const Raw& r) { return Planes1{{r}}; }
   static __device__ __forceinline__ De de(const f32x8& x) { return split2(x); }
@@ -159,7 +173,7 @@ template <> struct El<__bf16> {
   static __device__ __forceinline__ void score(f32x4& c, const Raw& a, const Raw& b) { c = mfma_bf(a, b, c); }
 };
 template <> struct El<_Float16> {
-  static constexpr int C = 64;
+  static constexpr int C = 64, PLANES = 1;
   typedef f16x8 Raw; typedef Planes2 In; typedef Planes2 De; typedef Planes3 Wt;
   static __device__ __forceinline__ f32x8 wide(const Raw& r) { return __builtin_convertvector(r, f32x8); }
   static __device__ __forceinline__ In in(const Raw& r) { return split2(wide(r)); }   // 11 significant bits: the two terms are exact
@@ -170,38 +184,39 @@ template <> struct El<_Float16> {
 
 __device__ __forceinline__ f32x8 join(const f32x4 a, const f32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// row `row` of a tile, reduction indices 32 s + {4g..4g+3, 16+4g..16+4g+3}; `tile` has PITCH bytes a row
+// q and k lie in LDS with the columns of every 32 in the order of the fragments, column (half, q, j) = 16 half + 4 q + j at place
+// 8 q + 4 half + j: a lane's {4g.., 16+4g..} are then neighbours.
+__device__ __forceinline__ constexpr int place4(int c4) { return (c4 & ~7) * 4 + 8 * (c4 & 3) + 4 * ((c4 >> 2) & 1); }   // of the four columns from 4 c4
+
+// row `row` of q or k, reduction indices 32 s + {4g..4g+3, 16+4g..16+4g+3}; `tile` has PITCH bytes a row and C rows a plane
 template <typename T, int PITCH>
 __device__ __forceinline__ typename El<T>::Raw row_frag(const char* tile, int row, int s, int g) {
-  const char* a = tile + row * PITCH + (32 * s + 4 * g) * (int)sizeof(T);
-  if constexpr (sizeof(T) == 4) {
-    return join(*reinterpret_cast<const f32x4*>(a), *reinterpret_cast<const f32x4*>(a + 64));
-  } else {
-    const u32x2 lo = *reinterpret_cast<const u32x2*>(a), hi = *reinterpret_cast<const u32x2*>(a + 32);
-    return __builtin_bit_cast(typename El<T>::Raw, __builtin_shufflevector(lo, hi, 0, 1, 2, 3));
-  }
-}
-// column col0 + lane % 16 of a tile, tokens 32 s + {4g.., 16+4g..}.  The whole wave takes part.
-template <typename T, int PITCH>
-__device__ __forceinline__ typename El<T>::Raw col_frag(const char* tile, int s, int col0, int lane) {
-  const int g = lane >> 4;
-  if constexpr (sizeof(T) == 4) {
-    const char* a = tile + (32 * s + 4 * g) * PITCH + (col0 + (lane & 15)) * 4;
-    f32x8 x;
+  const char* a = tile + row * PITCH + (32 * s + 8 * g) * 2;
+  if constexpr (El<T>::PLANES == 3) {
+    Planes3 r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = *reinterpret_cast<const float*>(a + e * PITCH);
-      x[4 + e] = *reinterpret_cast<const float*>(a + (16 + e) * PITCH);
-    }
-    return x;
-  } else {
-    // each lane names 8 bytes of a 4 x 16 block (row lane % 16 / 4, columns 4 (lane % 4)..); lane l gets column l of the block
-    typedef s16x4 __attribute__((address_space(3))) * lds_p;
-    const char* a = tile + (32 * s + 4 * g + ((lane >> 2) & 3)) * PITCH + (col0 + 4 * (lane & 3)) * 2;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 16 * PITCH));
-    return __builtin_bit_cast(typename El<T>::Raw, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
+    for (int q = 0; q < 3; ++q) r.p[q] = *reinterpret_cast<const bf16x8*>(a + q * El<T>::C * PITCH);
+    return r;
+  } else return __builtin_bit_cast(typename El<T>::Raw, *reinterpret_cast<const u32x4*>(a));
+}
+// column col0 + lane % 16 (col0 a multiple of 16), tokens 32 s + {4g.., 16+4g..}.  The whole wave takes part.
+template <int PITCH> __device__ __forceinline__ u32x4 transposed(const char* a) {
+  typedef s16x4 __attribute__((address_space(3))) * lds_p;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(a + 16 * PITCH));
+  return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+template <typename T, int PITCH, bool PLACED>
+__device__ __forceinline__ typename El<T>::Raw col_frag(const char* tile, int s, int col0, int lane) {
+  // each lane names 8 bytes of a 4 x 16 block (row lane % 16 / 4, columns 4 (lane % 4)..); lane l gets column l of the block
+  const int c = PLACED ? place4(col0 / 4 + (lane & 3)) : col0 + 4 * (lane & 3);
+  const char* a = tile + (32 * s + 4 * (lane >> 4) + ((lane >> 2) & 3)) * PITCH + c * 2;
+  if constexpr (El<T>::PLANES == 3) {
+    Planes3 r;
+#pragma unroll
+    for (int q = 0; q < 3; ++q) r.p[q] = __builtin_bit_cast(bf16x8, transposed<PITCH>(a + q * El<T>::C * PITCH));
+    return r;
+  } else return __builtin_bit_cast(typename El<T>::Raw, transposed<PITCH>(a));
 }
 
 // largest exponent pattern among the elements of a 16-byte unit, kept as a running maximum
@@ -243,56 +258,83 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const f32x4 x
 
 // A [C][W] tile of tokens t .. t+n-1, columns c0 .. c0+W-1 (zero beyond `dim` and n): 16-byte units, unit u of a thread in its
 // registers between the load and the write to LDS.
-template <typename T, int C, int W, int NTH>
+template <typename T, int C, int W, int NTH, bool PLACED>
 struct Stage {
-  static constexpr int E = 16 / (int)sizeof(T), UPR = W / E, UNITS = C * UPR, U = (UNITS + NTH - 1) / NTH, PITCH = W * (int)sizeof(T) + 16;
+  static constexpr int E = 16 / (int)sizeof(T), UPR = W / E, UNITS = C * UPR, U = UNITS / NTH, PITCH = W * 2 + 16, ROWS = NTH / UPR, BYTES = C * PITCH * El<T>::PLANES;
+  static_assert(UNITS % NTH == 0 && NTH % UPR == 0, "whole units per thread, whole rows per pass");
   u32x4 r[U];
-  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t step, int n, int c0, int dim, int vec, int tid) {
+  // p: the thread's first unit at the chunk's first token; its others lie ROWS tokens apart in the same columns, of which `cols` are
+  // inside the row.  Addresses need only the element's alignment.
+  template <bool VEC> __device__ __forceinline__ void load(const T* __restrict__ p, int64_t step, int n, int cols, int dim, int tid) {
+    const int row = tid / UPR;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = tid + NTH * i, row = u / UPR, c = c0 + (u % UPR) * E;
       u32x4 w = {0u, 0u, 0u, 0u};
-      if (row < n && c < dim) {                      // row < n <= C also keeps the unit inside the tile
-        const T* p = base + row * step + c;
-        if (vec) w = *reinterpret_cast<const u32x4*>(p);
-        else {
-          T x[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) x[e] = c + e < dim ? p[e] : (T)0.0f;
-          __builtin_memcpy(&w, x, 16);
+      if (row + ROWS * i < n && cols > 0) {          // row < n <= C also keeps the unit inside the tile
+        const T* q = p + step * (ROWS * i);
+        if constexpr (VEC) w = *reinterpret_cast<const u32x4*>(q);
+        else if (cols >= E || dim >= E) {            // a row's last, cut unit: the 16 bytes that end with the row, moved down
+          const int over = cols < E ? E - cols : 0;
+          __builtin_memcpy(&w, q - over, 16);
+          if (over) w = down(w, over * (int)sizeof(T) * 8);
+        } else {
+          for (int e = 0; e < cols; ++e) {
+            if constexpr (sizeof(T) == 4) w[e] = __builtin_bit_cast(unsigned, q[e]);
+            else w[e / 2] |= (unsigned)__builtin_bit_cast(unsigned short, q[e]) << (16 * (e & 1));
+          }
         }
       }
       r[i] = w;
     }
   }
+  static __device__ __forceinline__ u32x4 down(const u32x4 w, int bits) {   // 0 < bits < 128
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    u64x2 v = __builtin_bit_cast(u64x2, w);
+    if (bits >= 64) { v[0] = v[1]; v[1] = 0; bits -= 64; }
+    if (bits) { v[0] = v[0] >> bits | v[1] << (64 - bits); v[1] >>= bits; }
+    return __builtin_bit_cast(u32x4, v);
+  }
   __device__ __forceinline__ void store(char* tile, int tid, Peak<T>& peak) const {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = tid + NTH * i;
-      if (UNITS % NTH == 0 || u < UNITS) {
-        peak.see(r[i]);
-        *reinterpret_cast<u32x4*>(tile + (u / UPR) * PITCH + (u % UPR) * 16) = r[i];
+      peak.see(r[i]);
+      char* q = tile + (tid / UPR + ROWS * i) * PITCH;
+      const int cu = tid % UPR;
+      if constexpr (sizeof(T) == 4) {                // three exact bf16 terms, a plane each
+        const Planes3 x = split3(__builtin_bit_cast(f32x8, __builtin_shufflevector(r[i], r[i], 0, 1, 2, 3, 0, 1, 2, 3)));
+        q += (PLACED ? place4(cu) : 4 * cu) * 2;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(q + k * C * PITCH) = __builtin_shufflevector(__builtin_bit_cast(u32x4, x.p[k]), u32x4{}, 0, 1);
+      } else if constexpr (!PLACED) *reinterpret_cast<u32x4*>(q + cu * 16) = r[i];
+      else {
+        *reinterpret_cast<u32x2*>(q + place4(2 * cu) * 2) = u32x2{r[i][0], r[i][1]};
+        *reinterpret_cast<u32x2*>(q + place4(2 * cu + 1) * 2) = u32x2{r[i][2], r[i][3]};
       }
     }
   }
 };
 
+#ifndef MIN_WAVES
+#define MIN_WAVES 2
+#endif
 // DP: both widths padded; NT: 16-column tiles of the values per wave; STATE: only the segment's own contribution to the state
-template <typename T, int DP, int NT, bool STATE>
-__global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const ScanP p) {
+template <typename T, int DP, int NT, bool STATE, bool VEC>
+__global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(const ScanP p) {
   typedef El<T> X;
   typedef typename X::Raw Raw;
   typedef typename X::In In;
   typedef typename X::De De;
-  constexpr int C = X::C, WAVES = DP == 32 ? 2 : 4, NTH = WAVES * 64, DVB = WAVES * NT * 16;
+  constexpr int C = X::C, WAVES = DP / 16 / NT, NTH = WAVES * 64, DVB = WAVES * NT * 16;
   static_assert(DVB <= DP, "value slice");
   constexpr int KT = DP / 16, KS = DP / 32, CT = C / 16, JS = C / 32;
-  typedef Stage<T, C, DP, NTH> SQ;
-  typedef Stage<T, C, DVB, NTH> SV;
-  __shared__ __attribute__((aligned(16))) char lq[STATE ? 16 : C * SQ::PITCH];
-  __shared__ __attribute__((aligned(16))) char lk[C * SQ::PITCH];
-  __shared__ __attribute__((aligned(16))) char lv[C * SV::PITCH];
-  __shared__ __attribute__((aligned(16))) float wj[C];
+  typedef Stage<T, C, DP, NTH, true> SQ;
+  typedef Stage<T, C, DVB, NTH, false> SV;
+  __shared__ __attribute__((aligned(16))) char lq[STATE ? 16 : SQ::BYTES];
+  __shared__ __attribute__((aligned(16))) char lk[SQ::BYTES];
+  __shared__ __attribute__((aligned(16))) char lv[SV::BYTES];
+  __shared__ __attribute__((aligned(16))) float wj[C];   // per token of the chunk: weight of its k v^T in the state after the chunk,
+  __shared__ float rj[C];                                // weight of the state on entry in its output (0: a reset lies between),
+  __shared__ __attribute__((aligned(16))) int seg[C];    // number of resets before it reads
   __shared__ int wild[2];
 
   const Role& R = p.role[blockIdx.z];
@@ -303,10 +345,12 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
   const int c0 = vt * DVB, cw = c0 + wave * NT * 16;      // first value column of the block, of the wave
   if (c0 >= R.dv) return;
   const double l2 = log2_decay(p.log_decay, h);
-  const int off = R.off, dq = R.dq, dv = R.dv, vec = R.vec;
-  const T* qb = static_cast<const T*>(R.q) + b * R.qs[0] + h * R.qs[2];
-  const T* kb = static_cast<const T*>(R.k) + b * R.ks[0] + h * R.ks[2];
-  const T* vb = static_cast<const T*>(R.v) + b * R.vs[0] + h * R.vs[2];
+  const int off = R.off, dq = R.dq, dv = R.dv;
+  // the thread's first unit of each operand: column and token offset are its own, the chunk's first token is added per chunk
+  const int cq = (tid % SQ::UPR) * SQ::E, cv = c0 + (tid % SV::UPR) * SV::E, nq = dq - cq, nv = dv - cv;
+  const T* qb = static_cast<const T*>(R.q) + b * R.qs[0] + h * R.qs[2] + (tid / SQ::UPR) * R.qs[1] + cq;
+  const T* kb = static_cast<const T*>(R.k) + b * R.ks[0] + h * R.ks[2] + (tid / SQ::UPR) * R.ks[1] + cq;
+  const T* vb = static_cast<const T*>(R.v) + b * R.vs[0] + h * R.vs[2] + (tid / SV::UPR) * R.vs[1] + cv;
   T* ob = STATE ? nullptr : static_cast<T*>(R.out) + b * R.os[0] + h * R.os[2];
   const uint8_t* rb = R.resets ? R.resets + b * R.rs[0] : nullptr;
   const int64_t sz = (int64_t)dq * dv;
@@ -315,9 +359,9 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
   SV sv;
   int rbyte = 0;
   auto fetch = [&](int t, int n) {
-    if constexpr (!STATE) sq.load(qb + t * R.qs[1], R.qs[1], n, 0, dq, vec, tid);
-    sk.load(kb + t * R.ks[1], R.ks[1], n, 0, dq, vec, tid);
-    sv.load(vb + t * R.vs[1], R.vs[1], n, c0, dv, vec, tid);
+    if constexpr (!STATE) sq.template load<VEC>(qb + t * R.qs[1], R.qs[1], n, nq, dq, tid);
+    sk.template load<VEC>(kb + t * R.ks[1], R.ks[1], n, nq, dq, tid);
+    sv.template load<VEC>(vb + t * R.vs[1], R.vs[1], n, nv, dv, tid);
     rbyte = (rb && lane < n) ? rb[(t + lane) * R.rs[1]] : 0;
   };
   int t = t0, n = min(C, t1 - t0);
@@ -341,15 +385,12 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
           S[kt][nt][r] = (s0 && row < dq && col < dv) ? s0[(int64_t)row * sr + (int64_t)col * sc] : 0.0f;
         }
   }
-  // decay weights of a lane: reading (token 16 it + m), and the scores' lambda^(i-j): inside a diagonal tile directly, between tiles
+  // decay weights of the scores, lambda^(i-j): inside a diagonal tile directly, between tiles
   // d + 1 apart as lambda^(16 d + m + 1) * lambda^(15 - (4g + r)), both exponents non-negative
-  float rd[CT], ai[CT], bj[4], dg[4];
+  float ai[CT], bj[4], dg[4];
   if constexpr (!STATE) {
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      rd[i] = decay_pow(l2, 16 * i + m + off) * R.oscale;
-      ai[i] = decay_pow(l2, 16 * i + m + 1) * R.wscale * R.oscale;
-    }
+    for (int i = 0; i + 1 < CT; ++i) ai[i] = decay_pow(l2, 16 * i + m + 1) * R.wscale * R.oscale;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       bj[r] = decay_pow(l2, 15 - (4 * g + r));
@@ -366,10 +407,14 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
     // ---- stage the chunk
     const uint64_t rm = __ballot(rbyte != 0);
     const bool special = n != C || rm != 0;
-    if (special || !plain_w) {                          // weight of token j in the state after the chunk
+    if (special || !plain_w) {
       if (tid < C) {
         const uint64_t mj = (off ? (2ull << tid) : (1ull << tid)) - 1;
         wj[tid] = (tid < n && (rm & ~mj) == 0) ? decay_pow(l2, n - off - tid) * R.wscale : 0.0f;
+        if constexpr (!STATE) {
+          rj[tid] = (rm & mj) == 0 ? decay_pow(l2, tid + off) * R.oscale : 0.0f;
+          seg[tid] = __builtin_popcountll(rm & mj);
+        }
       }
       plain_w = !special;
     }
@@ -392,7 +437,8 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
     const int tn = t + n, nn = tn < careful ? 1 : min(C, t1 - tn);
     if (tn < t1) fetch(tn, nn);
 
-    // ---- the chunk's products
+    // ---- the chunk's products (none for a wave whose columns are padding)
+    if (cw < dv) {
     De sf[KS][NT];
     if constexpr (!STATE) {
 #pragma unroll
@@ -400,22 +446,16 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sf[s][nt] = X::de(join(S[2 * s][nt], S[2 * s + 1][nt]));
     }
-    In vin[JS][NT];
-    typename X::Wt vw[JS][NT];
-#pragma unroll
-    for (int s = 0; s < JS; ++s) {
-      const f32x8 w = join(*reinterpret_cast<const f32x4*>(wj + 32 * s + 4 * g), *reinterpret_cast<const f32x4*>(wj + 32 * s + 16 + 4 * g));
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const Raw r = col_frag<T, SV::PITCH>(lv, s, wave * NT * 16 + 16 * nt, lane);
-        if constexpr (!STATE) vin[s][nt] = X::in(r);
-        vw[s][nt] = X::wt(X::wide(r) * w);
-      }
-    }
     if constexpr (!STATE) {
+      In vin[JS][NT];
+#pragma unroll
+      for (int s = 0; s < JS; ++s)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) vin[s][nt] = X::in(col_frag<T, SV::PITCH, false>(lv, s, wave * NT * 16 + 16 * nt, lane));
 #pragma unroll
       for (int it = 0; it < CT; ++it) {
         if (16 * it >= n) break;
+        asm volatile("" ::: "memory");                   // k is read from LDS again for every 16 rows: kept, it would cost half the waves
         Raw qf[KS];
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = row_frag<T, SQ::PITCH>(lq, 16 * it + m, s, g);
@@ -424,17 +464,17 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
         for (int nt = 0; nt < NT; ++nt) o[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
+          if (32 * s >= dq) break;
           const In qi = X::in(qf[s]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma(o[nt], sf[s][nt], qi);
         }
         const int i = 16 * it + m;
-        const uint64_t mi = (off ? (2ull << i) : (1ull << i)) - 1;
-        const bool reads = (rm & mi) == 0;               // no reset between the state on entry and token i
+        const float rd = rj[i];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[nt][r] = reads ? o[nt][r] * rd[it] : 0.0f;
+          for (int r = 0; r < 4; ++r) o[nt][r] = rd != 0.0f ? o[nt][r] * rd : 0.0f;
 #pragma unroll
         for (int s = 0; s < JS; ++s) {
           if (2 * s > it) break;
@@ -445,19 +485,17 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
             if (jt <= it) {
 #pragma unroll
-              for (int ks = 0; ks < KS; ++ks) X::score(a, row_frag<T, SQ::PITCH>(lk, 16 * jt + m, ks, g), qf[ks]);
+              for (int ks = 0; ks < KS; ++ks)
+                if (32 * ks < dq) X::score(a, row_frag<T, SQ::PITCH>(lk, 16 * jt + m, ks, g), qf[ks]);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 if (jt == it) a[r] = m >= 4 * g + r ? a[r] * dg[r] : 0.0f;
                 else a[r] = a[r] * (ai[it - jt - 1] * bj[r]);
               }
               if (rm) {
+                const int si = seg[i];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const int j = 16 * jt + 4 * g + r;
-                  const uint64_t mj = (off ? (2ull << j) : (1ull << j)) - 1;
-                  if (rm & mi & ~mj) a[r] = 0.0f;
-                }
+                for (int r = 0; r < 4; ++r) a[r] = seg[16 * jt + 4 * g + r] == si ? a[r] : 0.0f;
               }
             }
             pt[u] = a;
@@ -476,6 +514,7 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
       }
     }
     // ---- the state after the chunk
+    asm volatile("" ::: "memory");
     const float dec = n == C ? pC : decay_pow(l2, n);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
@@ -486,12 +525,18 @@ __global__ __launch_bounds__((DP == 32 ? 2 : 4) * 64) void scan_kernel(const Sca
 #pragma unroll
     for (int s = 0; s < JS; ++s) {
       if (32 * s >= n || (n == 1 && rm && !off)) break;   // a lone token whose write its own reset drops: zero times an infinity is none
+      const f32x8 w = join(*reinterpret_cast<const f32x4*>(wj + 32 * s + 4 * g), *reinterpret_cast<const f32x4*>(wj + 32 * s + 16 + 4 * g));
+      typename X::Wt vw[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) vw[nt] = X::wt(X::wide(col_frag<T, SV::PITCH, false>(lv, s, wave * NT * 16 + 16 * nt, lane)) * w);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const In kc = X::in(col_frag<T, SQ::PITCH>(lk, s, 16 * kt, lane));
+        if (16 * kt >= dq) break;
+        const In kc = X::in(col_frag<T, SQ::PITCH, true>(lk, s, 16 * kt, lane));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma(S[kt][nt], kc, vw[s][nt]);
+        for (int nt = 0; nt < NT; ++nt) mma(S[kt][nt], kc, vw[nt]);
       }
+    }
     }
     any_reset |= rm != 0;
     __syncthreads();                                     // every wave has read the tiles
@@ -632,18 +677,18 @@ int check_pointers(const mrl_attention* p, const char* what) {
   return MRL_OK;
 }
 
-// How the work is cut.  Blocks per CU matter, not their number of tokens: with fewer than 512 blocks (two per CU) the tokens are
-// split into segments of at least four chunks, whose states are computed first, joined, and handed to the second pass.
+// How the work is cut: 2048 waves (two a SIMD) keep the card busy, a block has one for every 16 value columns.  With fewer blocks the
+// tokens are split into segments of whole chunks, whose states are computed first, joined, and handed to the second pass.
 Plan plan_of(const mrl_attention* p, int roles) {
   Plan r;
   const int d = std::max(p->dim_k, p->dim_v);
-  r.dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
-  r.nt = r.dp == 128 ? 2 : 1;
+  r.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128;
+  r.nt = 1;
   r.v_tiles = 1;
   const int C = chunk_of(p->dtype);
   const int64_t blocks = std::max<int64_t>(1, p->batch * p->heads * r.v_tiles * roles);
   const int64_t chunks = cdiv(p->steps, C);
-  int64_t splits = std::min<int64_t>(cdiv(512, blocks), chunks / 4);
+  int64_t splits = std::min<int64_t>(cdiv(2048 / (r.dp / 16), blocks), chunks);
   if (splits < 2) splits = 1;
   const int64_t per = std::max<int64_t>(1, cdiv(chunks, splits));
   r.seg = (int)(per * C);
@@ -659,19 +704,27 @@ int64_t ws_bytes(const mrl_attention* p, const Plan& pl, int roles) {
   return role_floats(p, pl) * roles * 4 + (int64_t)roles * pl.n_splits * p->batch * p->heads * 4;
 }
 
-template <typename T, int DP, int NT> void launch(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
-  const unsigned gx = (unsigned)(a.BH * pl.v_tiles), nth = DP == 32 ? 128 : 256;
+template <typename T, int DP, int NT, bool VEC> void launch_as(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
+  const unsigned gx = (unsigned)(a.BH * pl.v_tiles), nth = DP / 16 / NT * 64;
   if (pl.n_splits > 1) {
-    hipLaunchKernelGGL((scan_kernel<T, DP, NT, true>), dim3(gx, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
+    hipLaunchKernelGGL((scan_kernel<T, DP, NT, true, VEC>), dim3(gx, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
     const int64_t sz = (int64_t)a.role[0].dq * a.role[0].dv;
     hipLaunchKernelGGL(prefix_kernel, dim3((unsigned)cdiv(sz, 256), a.BH, roles), dim3(256), 0, st, a);
   }
-  hipLaunchKernelGGL((scan_kernel<T, DP, NT, false>), dim3(gx, pl.n_splits, roles), dim3(nth), 0, st, a);
+  hipLaunchKernelGGL((scan_kernel<T, DP, NT, false, VEC>), dim3(gx, pl.n_splits, roles), dim3(nth), 0, st, a);
 }
 template <typename T> void launch(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
-  if (pl.dp == 32) launch<T, 32, 1>(a, pl, roles, st);
-  else if (pl.dp == 64) launch<T, 64, 1>(a, pl, roles, st);
-  else launch<T, 128, 2>(a, pl, roles, st);
+  bool vec = true;
+  for (int i = 0; i < roles; ++i) vec = vec && a.role[i].vec;
+  auto go = [&](auto v) {
+    constexpr bool VEC = decltype(v)::value;
+    if (pl.dp == 32) launch_as<T, 32, 1, VEC>(a, pl, roles, st);
+    else if (pl.dp == 64) launch_as<T, 64, 1, VEC>(a, pl, roles, st);
+    else if (pl.dp == 96) launch_as<T, 96, 1, VEC>(a, pl, roles, st);
+    else launch_as<T, 128, 1, VEC>(a, pl, roles, st);
+  };
+  if (vec) go(std::true_type());
+  else go(std::false_type());
 }
 int dispatch(const mrl_attention* p, ScanP& a, const Plan& pl, int roles, void* ws, int64_t bytes, void* stream, const char* what) {
   const int64_t need = ws_bytes(p, pl, roles);
