@@ -317,9 +317,12 @@ struct Stage {
 #ifndef MIN_WAVES
 #define MIN_WAVES 2
 #endif
+#ifndef MIN_WAVES_S
+#define MIN_WAVES_S 3
+#endif
 // DP: both widths padded; NT: 16-column tiles of the values per wave; STATE: only the segment's own contribution to the state
-template <typename T, int DP, int NT, bool STATE, bool VEC>
-__global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(const ScanP p) {
+template <typename T, int DP, int NT, bool STATE, bool VEC, bool SINGLE>
+__global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES) void scan_kernel(const ScanP p) {
   typedef El<T> X;
   typedef typename X::Raw Raw;
   typedef typename X::In In;
@@ -333,6 +336,7 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(cons
   __shared__ __attribute__((aligned(16))) char lk[SQ::BYTES];
   __shared__ __attribute__((aligned(16))) char lv[SV::BYTES];
   __shared__ __attribute__((aligned(16))) float wj[C];   // per token of the chunk: weight of its k v^T in the state after the chunk,
+  __shared__ float pw[C + 1];                            // lambda^n
   __shared__ float rj[C];                                // weight of the state on entry in its output (0: a reset lies between),
   __shared__ __attribute__((aligned(16))) int seg[C];    // number of resets before it reads
   __shared__ int wild[2];
@@ -382,26 +386,27 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(cons
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int row = 16 * kt + 4 * g + r, col = cw + 16 * nt + m;
-          S[kt][nt][r] = (s0 && row < dq && col < dv) ? s0[(int64_t)row * sr + (int64_t)col * sc] : 0.0f;
+          S[kt][nt][r] = (s0 && row < dq && col < dv) ? s0[(unsigned)(row * sr + col * sc)] : 0.0f;
         }
   }
-  // decay weights of the scores, lambda^(i-j): inside a diagonal tile directly, between tiles
-  // d + 1 apart as lambda^(16 d + m + 1) * lambda^(15 - (4g + r)), both exponents non-negative
+  // lambda^n for every distance inside a chunk; scores weigh by lambda^(i-j): inside a diagonal tile directly, between tiles d + 1 apart
+  // as lambda^(16 d + m + 1) * lambda^(15 - (4g + r)), both exponents non-negative
+  for (int i = tid; i <= C; i += NTH) pw[i] = decay_pow(l2, i);
+  if (tid < 2) wild[tid] = 0;
+  __syncthreads();
+  const float scale = R.wscale * R.oscale, pC = pw[C];
   float ai[CT], bj[4], dg[4];
   if constexpr (!STATE) {
 #pragma unroll
-    for (int i = 0; i + 1 < CT; ++i) ai[i] = decay_pow(l2, 16 * i + m + 1) * R.wscale * R.oscale;
+    for (int i = 0; i + 1 < CT; ++i) ai[i] = pw[16 * i + m + 1] * scale;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      bj[r] = decay_pow(l2, 15 - (4 * g + r));
-      dg[r] = decay_pow(l2, m - (4 * g + r)) * R.wscale * R.oscale;
+      bj[r] = pw[15 - (4 * g + r)];
+      dg[r] = pw[max(m - (4 * g + r), 0)] * scale;
     }
   }
-  const float pC = decay_pow(l2, C);
   bool plain_w = false;
   int any_reset = 0, careful = t0, turn = 0;
-  if (tid < 2) wild[tid] = 0;
-  __syncthreads();
 
   while (t < t1) {
     // ---- stage the chunk
@@ -410,9 +415,9 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(cons
     if (special || !plain_w) {
       if (tid < C) {
         const uint64_t mj = (off ? (2ull << tid) : (1ull << tid)) - 1;
-        wj[tid] = (tid < n && (rm & ~mj) == 0) ? decay_pow(l2, n - off - tid) * R.wscale : 0.0f;
+        wj[tid] = (tid < n && (rm & ~mj) == 0) ? pw[max(n - off - tid, 0)] * R.wscale : 0.0f;
         if constexpr (!STATE) {
-          rj[tid] = (rm & mj) == 0 ? decay_pow(l2, tid + off) * R.oscale : 0.0f;
+          rj[tid] = (rm & mj) == 0 ? pw[tid + off] * R.oscale : 0.0f;
           seg[tid] = __builtin_popcountll(rm & mj);
         }
       }
@@ -435,7 +440,7 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(cons
       continue;
     }
     const int tn = t + n, nn = tn < careful ? 1 : min(C, t1 - tn);
-    if (tn < t1) fetch(tn, nn);
+    if (SINGLE ? nn == 1 && tn < t1 : tn < t1) fetch(tn, nn);   // (a single chunk has a next one only when its tokens are walked)
 
     // ---- the chunk's products (none for a wave whose columns are padding)
     if (cw < dv) {
@@ -485,8 +490,10 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(cons
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
             if (jt <= it) {
 #pragma unroll
-              for (int ks = 0; ks < KS; ++ks)
+              for (int ks = 0; ks < KS; ++ks) {
+                if (X::PLANES == 3 || ks == 0) asm volatile("" ::: "memory");    // fragments of k are read as they are needed, not all at once
                 if (32 * ks < dq) X::score(a, row_frag<T, SQ::PITCH>(lk, 16 * jt + m, ks, g), qf[ks]);
+              }
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 if (jt == it) a[r] = m >= 4 * g + r ? a[r] * dg[r] : 0.0f;
@@ -515,7 +522,7 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(cons
     }
     // ---- the state after the chunk
     asm volatile("" ::: "memory");
-    const float dec = n == C ? pC : decay_pow(l2, n);
+    const float dec = n == C ? pC : pw[n];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -556,7 +563,7 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, MIN_WAVES) void scan_kernel(cons
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int row = 16 * kt + 4 * g + r, col = cw + 16 * nt + m;
-          if (row < dq && col < dv) s1[(int64_t)row * sr + (int64_t)col * sc] = S[kt][nt][r];
+          if (row < dq && col < dv) s1[(unsigned)(row * sr + col * sc)] = S[kt][nt][r];
         }
   }
   if (STATE && vt == 0 && tid == 0) p.flags[((int64_t)blockIdx.z * p.n_splits + split) * p.BH + bh] = any_reset;
@@ -707,11 +714,12 @@ int64_t ws_bytes(const mrl_attention* p, const Plan& pl, int roles) {
 template <typename T, int DP, int NT, bool VEC> void launch_as(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
   const unsigned gx = (unsigned)(a.BH * pl.v_tiles), nth = DP / 16 / NT * 64;
   if (pl.n_splits > 1) {
-    hipLaunchKernelGGL((scan_kernel<T, DP, NT, true, VEC>), dim3(gx, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
+    hipLaunchKernelGGL((scan_kernel<T, DP, NT, true, VEC, false>), dim3(gx, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
     const int64_t sz = (int64_t)a.role[0].dq * a.role[0].dv;
     hipLaunchKernelGGL(prefix_kernel, dim3((unsigned)cdiv(sz, 256), a.BH, roles), dim3(256), 0, st, a);
   }
-  hipLaunchKernelGGL((scan_kernel<T, DP, NT, false, VEC>), dim3(gx, pl.n_splits, roles), dim3(nth), 0, st, a);
+  if (a.T <= El<T>::C) hipLaunchKernelGGL((scan_kernel<T, DP, NT, false, VEC, true>), dim3(gx, 1, roles), dim3(nth), 0, st, a);
+  else hipLaunchKernelGGL((scan_kernel<T, DP, NT, false, VEC, false>), dim3(gx, pl.n_splits, roles), dim3(nth), 0, st, a);
 }
 template <typename T> void launch(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
   bool vec = true;

@@ -30,7 +30,8 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
   const bf16x2 v = {(__bf16)a, (__bf16)b};
   return __builtin_bit_cast(unsigned, v);
 }
-__device__ __forceinline__ float half_lo(unsigned pk) { return __uint_as_float(pk << 16); }
+// (v_perm for the low half: a shift makes the compiler convert that element a second time by itself)
+__device__ __forceinline__ float half_lo(unsigned pk) { return __uint_as_float(__builtin_amdgcn_perm(pk, 0u, 0x05040c0cu)); }
 __device__ __forceinline__ float half_hi(unsigned pk) { return __uint_as_float(pk & 0xffff0000u); }
 
 // Activations and their derivatives at z, in fp32.  `act` is uniform over the launch.  The logistic function uses the hardware's
