@@ -8,8 +8,8 @@
 // dk = scan(v, do; q), dv = scan(k, q; do), whose state is the gradient of S (the last one's end is the initial state's gradient).
 // Backwards the decay follows a token's write instead of preceding it (`off` 0 instead of 1).  One kernel serves all four.
 //
-// Layout: one block per (batch row, head, segment of the tokens, slice of the value columns), 2 or 4 waves, each wave owning 16
-// (or 32) value columns and all rows of S in MFMA accumulators for the whole segment.  The products are arranged so that every
+// Layout: one block per (batch row, head, segment of the tokens), one wave for every 16 value columns, which holds all rows of its
+// columns of S in MFMA accumulators for the whole segment.  The products are arranged so that every
 // intermediate is the next product's operand where it lies: with 16x16x32 MFMAs a lane's accumulators of two stacked 16-row tiles
 // are rows {4g..4g+3, 16+4g..16+4g+3} of its column (g = lane / 16), and any order of the reduction index serves as long as both
 // operands share it, so S and P^T go from accumulators to operands without LDS; row-major operands lie in LDS in that order and are
@@ -46,7 +46,7 @@ struct Role {
   int dq, dv;                    // reduction width (q, k), output width (v)
   int off;                       // decays between the state on entry and the first token's reading
   float oscale, wscale;          // factor of the outputs; factor of every k v^T
-  int vec;                       // all rows of q, k, v are whole 16-byte units on 16-byte addresses
+  int vec;                       // all rows of q, k, v lie on 16-byte addresses
   int64_t ws;                    // this role's place in the workspace, floats
 };
 
@@ -265,14 +265,14 @@ struct Stage {
   u32x4 r[U];
   // p: the thread's first unit at the chunk's first token; its others lie ROWS tokens apart in the same columns, of which `cols` are
   // inside the row.  Addresses need only the element's alignment.
-  template <bool VEC> __device__ __forceinline__ void load(const T* __restrict__ p, int64_t step, int n, int cols, int dim, int tid) {
+  template <bool FULL> __device__ __forceinline__ void load(const T* __restrict__ p, int64_t step, int n, int cols, int dim, int tid) {
     const int row = tid / UPR;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       u32x4 w = {0u, 0u, 0u, 0u};
-      if (row + ROWS * i < n && cols > 0) {          // row < n <= C also keeps the unit inside the tile
+      if (row + ROWS * i < n && (FULL || cols > 0)) {          // row < n <= C also keeps the unit inside the tile
         const T* q = p + step * (ROWS * i);
-        if constexpr (VEC) w = *reinterpret_cast<const u32x4*>(q);
+        if constexpr (FULL) w = *reinterpret_cast<const u32x4*>(q);
         else if (cols >= E || dim >= E) {            // a row's last, cut unit: the 16 bytes that end with the row, moved down
           const int over = cols < E ? E - cols : 0;
           __builtin_memcpy(&w, q - over, 16);
@@ -314,24 +314,18 @@ struct Stage {
   }
 };
 
-#ifndef MIN_WAVES
-#define MIN_WAVES 2
-#endif
-#ifndef MIN_WAVES_S
-#define MIN_WAVES_S 3
-#endif
-// DP: both widths padded; NT: 16-column tiles of the values per wave; STATE: only the segment's own contribution to the state
-template <typename T, int DP, int NT, bool STATE, bool VEC, bool SINGLE>
-__global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES) void scan_kernel(const ScanP p) {
+// DP: both widths padded; STATE: only the segment's own contribution to the state; FULL: both widths are DP and
+// all rows lie on 16-byte addresses; PACK: sequences of one chunk, several to a block, the next one's loads under way during the present one's products
+template <typename T, int DP, bool STATE, bool FULL, bool PACK>
+__global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
   typedef El<T> X;
   typedef typename X::Raw Raw;
   typedef typename X::In In;
   typedef typename X::De De;
-  constexpr int C = X::C, WAVES = DP / 16 / NT, NTH = WAVES * 64, DVB = WAVES * NT * 16;
-  static_assert(DVB <= DP, "value slice");
+  constexpr int C = X::C, WAVES = DP / 16, NTH = WAVES * 64;
   constexpr int KT = DP / 16, KS = DP / 32, CT = C / 16, JS = C / 32;
   typedef Stage<T, C, DP, NTH, true> SQ;
-  typedef Stage<T, C, DVB, NTH, false> SV;
+  typedef Stage<T, C, DP, NTH, false> SV;
   __shared__ __attribute__((aligned(16))) char lq[STATE ? 16 : SQ::BYTES];
   __shared__ __attribute__((aligned(16))) char lk[SQ::BYTES];
   __shared__ __attribute__((aligned(16))) char lv[SV::BYTES];
@@ -343,52 +337,65 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
 
   const Role& R = p.role[blockIdx.z];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int bh = blockIdx.x % p.BH, vt = blockIdx.x / p.BH, split = blockIdx.y;
-  const int b = bh / p.H, h = bh % p.H;
-  const int t0 = split * p.seg, t1 = min(p.T, t0 + p.seg);
-  const int c0 = vt * DVB, cw = c0 + wave * NT * 16;      // first value column of the block, of the wave
-  if (c0 >= R.dv) return;
+  const int split = blockIdx.y, t0 = split * p.seg, t1 = min(p.T, t0 + p.seg);
+  int bh = blockIdx.x;                                    // PACK: one of a run of (row, head), all of the same head
+  const int h = bh % p.H, cw = wave * 16;                 // first value column of the wave
   const double l2 = log2_decay(p.log_decay, h);
-  const int off = R.off, dq = R.dq, dv = R.dv;
-  // the thread's first unit of each operand: column and token offset are its own, the chunk's first token is added per chunk
-  const int cq = (tid % SQ::UPR) * SQ::E, cv = c0 + (tid % SV::UPR) * SV::E, nq = dq - cq, nv = dv - cv;
-  const T* qb = static_cast<const T*>(R.q) + b * R.qs[0] + h * R.qs[2] + (tid / SQ::UPR) * R.qs[1] + cq;
-  const T* kb = static_cast<const T*>(R.k) + b * R.ks[0] + h * R.ks[2] + (tid / SQ::UPR) * R.ks[1] + cq;
-  const T* vb = static_cast<const T*>(R.v) + b * R.vs[0] + h * R.vs[2] + (tid / SV::UPR) * R.vs[1] + cv;
-  T* ob = STATE ? nullptr : static_cast<T*>(R.out) + b * R.os[0] + h * R.os[2];
-  const uint8_t* rb = R.resets ? R.resets + b * R.rs[0] : nullptr;
+  const int off = R.off, dq = FULL ? DP : R.dq, dv = FULL ? DP : R.dv;
+  // the thread's first unit of each operand: column and token offset are its own, the rest is the block's
+  const int cq = (tid % SQ::UPR) * SQ::E, cv = (tid % SV::UPR) * SV::E, nq = dq - cq, nv = dv - cv;
+  const int64_t ql = (tid / SQ::UPR) * R.qs[1] + cq, kl = (tid / SQ::UPR) * R.ks[1] + cq, vl = (tid / SV::UPR) * R.vs[1] + cv;
   const int64_t sz = (int64_t)dq * dv;
 
   SQ sq, sk;
   SV sv;
   int rbyte = 0;
-  auto fetch = [&](int t, int n) {
-    if constexpr (!STATE) sq.template load<VEC>(qb + t * R.qs[1], R.qs[1], n, nq, dq, tid);
-    sk.template load<VEC>(kb + t * R.ks[1], R.ks[1], n, nq, dq, tid);
-    sv.template load<VEC>(vb + t * R.vs[1], R.vs[1], n, nv, dv, tid);
-    rbyte = (rb && lane < n) ? rb[(t + lane) * R.rs[1]] : 0;
+  auto fetch = [&](int bh, int t, int n) {
+    const int64_t b = bh / p.H;
+    if constexpr (!STATE) sq.template load<FULL>(static_cast<const T*>(R.q) + b * R.qs[0] + h * R.qs[2] + t * R.qs[1] + ql, R.qs[1], n, nq, dq, tid);
+    sk.template load<FULL>(static_cast<const T*>(R.k) + b * R.ks[0] + h * R.ks[2] + t * R.ks[1] + kl, R.ks[1], n, nq, dq, tid);
+    sv.template load<FULL>(static_cast<const T*>(R.v) + b * R.vs[0] + h * R.vs[2] + t * R.vs[1] + vl, R.vs[1], n, nv, dv, tid);
+    rbyte = (R.resets && lane < n) ? R.resets[b * R.rs[0] + (t + lane) * R.rs[1]] : 0;
   };
-  int t = t0, n = min(C, t1 - t0);
-  if (n > 0) fetch(t, n);
-
-  f32x4 S[KT][NT];
-  {
+  auto load_state = [&](int bh, f32x4 (&S)[KT]) {
     const float* s0 = nullptr;
     int sr = R.s_row, sc = R.s_col;
     if (!STATE) {
       if (split == 0) s0 = R.s0 ? R.s0 + bh * sz : nullptr;
       else { s0 = p.ws + R.ws + ((int64_t)(split - 1) * p.BH + bh) * sz; sr = dv; sc = 1; }
     }
+    if (FULL && s0 && sr == 1) {                          // transposed: a lane's four rows are neighbours
+      typedef f32x4 __attribute__((aligned(4))) unit;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) S[kt] = *reinterpret_cast<const unit*>(s0 + (unsigned)((cw + m) * sc + 16 * kt + 4 * g));
+      return;
+    }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * kt + 4 * g + r, col = cw + m;
+        S[kt][r] = (s0 && row < dq && col < dv) ? s0[(unsigned)(row * sr + col * sc)] : 0.0f;
+      }
+  };
+  auto store_state = [&](int bh, const f32x4 (&S)[KT]) {
+    float* s1 = nullptr;
+    int sr = R.s_row, sc = R.s_col;
+    if (STATE) { s1 = p.ws + R.ws + ((int64_t)split * p.BH + bh) * sz; sr = dv; sc = 1; }
+    else if (split == p.n_splits - 1) s1 = R.s1 ? R.s1 + bh * sz : nullptr;
+    if (!s1) return;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * kt + 4 * g + r, col = cw + 16 * nt + m;
-          S[kt][nt][r] = (s0 && row < dq && col < dv) ? s0[(unsigned)(row * sr + col * sc)] : 0.0f;
-        }
-  }
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * kt + 4 * g + r, col = cw + m;
+        if (row < dq && col < dv) s1[(unsigned)(row * sr + col * sc)] = S[kt][r];
+      }
+  };
+  int t = t0, n = min(C, t1 - t0);
+  if (n > 0) fetch(bh, t, n);
+  f32x4 S[KT], Sn[PACK ? KT : 1];
+  load_state(bh, S);
   // lambda^n for every distance inside a chunk; scores weigh by lambda^(i-j): inside a diagonal tile directly, between tiles d + 1 apart
   // as lambda^(16 d + m + 1) * lambda^(15 - (4g + r)), both exponents non-negative
   for (int i = tid; i <= C; i += NTH) pw[i] = decay_pow(l2, i);
@@ -405,14 +412,13 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
       dg[r] = pw[max(m - (4 * g + r), 0)] * scale;
     }
   }
-  bool plain_w = false;
+  int plain_n = 0;                                        // length of the chunk without resets that the tables stand for
   int any_reset = 0, careful = t0, turn = 0;
 
   while (t < t1) {
     // ---- stage the chunk
     const uint64_t rm = __ballot(rbyte != 0);
-    const bool special = n != C || rm != 0;
-    if (special || !plain_w) {
+    if (rm != 0 || plain_n != n) {
       if (tid < C) {
         const uint64_t mj = (off ? (2ull << tid) : (1ull << tid)) - 1;
         wj[tid] = (tid < n && (rm & ~mj) == 0) ? pw[max(n - off - tid, 0)] * R.wscale : 0.0f;
@@ -421,7 +427,7 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
           seg[tid] = __builtin_popcountll(rm & mj);
         }
       }
-      plain_w = !special;
+      plain_n = rm ? 0 : n;
     }
     Peak<T> peak;
     if constexpr (!STATE) sq.store(lq, tid, peak);
@@ -436,27 +442,27 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
       careful = t + n;
       n = 1;
       __syncthreads();
-      fetch(t, n);
+      fetch(bh, t, n);
       continue;
     }
     const int tn = t + n, nn = tn < careful ? 1 : min(C, t1 - tn);
-    if (SINGLE ? nn == 1 && tn < t1 : tn < t1) fetch(tn, nn);   // (a single chunk has a next one only when its tokens are walked)
+    const int next = PACK ? bh + (int)gridDim.x : p.BH;
+    if (tn < t1) fetch(bh, tn, nn);
+    else if (PACK && next < p.BH) {
+      fetch(next, t0, t1 - t0);
+      load_state(next, reinterpret_cast<f32x4(&)[KT]>(Sn));
+    }
 
     // ---- the chunk's products (none for a wave whose columns are padding)
     if (cw < dv) {
-    De sf[KS][NT];
     if constexpr (!STATE) {
+      De sf[KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KS; ++s) sf[s] = X::de(join(S[2 * s], S[2 * s + 1]));
+      In vin[JS];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sf[s][nt] = X::de(join(S[2 * s][nt], S[2 * s + 1][nt]));
-    }
-    if constexpr (!STATE) {
-      In vin[JS][NT];
-#pragma unroll
-      for (int s = 0; s < JS; ++s)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) vin[s][nt] = X::in(col_frag<T, SV::PITCH, false>(lv, s, wave * NT * 16 + 16 * nt, lane));
+      for (int s = 0; s < JS; ++s) vin[s] = X::in(col_frag<T, SV::PITCH, false>(lv, s, cw, lane));
+      const int64_t obase = (int64_t)(bh / p.H) * R.os[0] + h * R.os[2];
 #pragma unroll
       for (int it = 0; it < CT; ++it) {
         if (16 * it >= n) break;
@@ -464,22 +470,16 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
         Raw qf[KS];
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = row_frag<T, SQ::PITCH>(lq, 16 * it + m, s, g);
-        f32x4 o[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) o[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           if (32 * s >= dq) break;
-          const In qi = X::in(qf[s]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma(o[nt], sf[s][nt], qi);
+          mma(o, sf[s], X::in(qf[s]));
         }
         const int i = 16 * it + m;
         const float rd = rj[i];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[nt][r] = rd != 0.0f ? o[nt][r] * rd : 0.0f;
+        for (int r = 0; r < 4; ++r) o[r] = rd != 0.0f ? o[r] * rd : 0.0f;
 #pragma unroll
         for (int s = 0; s < JS; ++s) {
           if (2 * s > it) break;
@@ -508,15 +508,11 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
             pt[u] = a;
           }
           const De pf = X::de(join(pt[0], pt[1]));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma(o[nt], vin[s][nt], pf);
+          mma(o, vin[s], pf);
         }
         if (i < n) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int c = cw + 16 * nt + 4 * g;
-            store4<T>(ob + (int64_t)(t + i) * R.os[1] + c, o[nt], dv - c, (dv & 3) == 0);
-          }
+          const int c = cw + 4 * g;
+          store4<T>(static_cast<T*>(R.out) + obase + (t + i) * R.os[1] + c, o, dv - c, (dv & 3) == 0);
         }
       }
     }
@@ -526,22 +522,16 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[kt][nt][r] = rm ? 0.0f : S[kt][nt][r] * dec;
+      for (int r = 0; r < 4; ++r) S[kt][r] = rm ? 0.0f : S[kt][r] * dec;
 #pragma unroll
     for (int s = 0; s < JS; ++s) {
       if (32 * s >= n || (n == 1 && rm && !off)) break;   // a lone token whose write its own reset drops: zero times an infinity is none
       const f32x8 w = join(*reinterpret_cast<const f32x4*>(wj + 32 * s + 4 * g), *reinterpret_cast<const f32x4*>(wj + 32 * s + 16 + 4 * g));
-      typename X::Wt vw[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) vw[nt] = X::wt(X::wide(col_frag<T, SV::PITCH, false>(lv, s, wave * NT * 16 + 16 * nt, lane)) * w);
+      const typename X::Wt vw = X::wt(X::wide(col_frag<T, SV::PITCH, false>(lv, s, cw, lane)) * w);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         if (16 * kt >= dq) break;
-        const In kc = X::in(col_frag<T, SQ::PITCH, true>(lk, s, 16 * kt, lane));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma(S[kt][nt], kc, vw[nt]);
+        mma(S[kt], X::in(col_frag<T, SQ::PITCH, true>(lk, s, 16 * kt, lane)), vw);
       }
     }
     }
@@ -549,24 +539,17 @@ __global__ __launch_bounds__(DP / 16 / NT * 64, SINGLE ? MIN_WAVES_S : MIN_WAVES
     __syncthreads();                                     // every wave has read the tiles
     t = tn;
     n = nn;
+    if (PACK && tn >= t1 && next < p.BH) {
+      store_state(bh, S);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) S[kt] = Sn[PACK ? kt : 0];
+      bh = next;
+      t = careful = t0;
+      n = t1 - t0;
+    }
   }
-
-  float* s1 = nullptr;
-  int sr = R.s_row, sc = R.s_col;
-  if (STATE) { s1 = p.ws + R.ws + ((int64_t)split * p.BH + bh) * sz; sr = dv; sc = 1; }
-  else if (split == p.n_splits - 1) s1 = R.s1 ? R.s1 + bh * sz : nullptr;
-  if (s1) {
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * kt + 4 * g + r, col = cw + 16 * nt + m;
-          if (row < dq && col < dv) s1[(unsigned)(row * sr + col * sc)] = S[kt][nt][r];
-        }
-  }
-  if (STATE && vt == 0 && tid == 0) p.flags[((int64_t)blockIdx.z * p.n_splits + split) * p.BH + bh] = any_reset;
+  store_state(bh, S);
+  if (STATE && tid == 0) p.flags[((int64_t)blockIdx.z * p.n_splits + split) * p.BH + bh] = any_reset;
 }
 
 // Between the two passes over a split sequence: the segments' own contributions become the states on entry.  Slot s holds segment
@@ -662,7 +645,7 @@ __global__ __launch_bounds__(256) void step_kernel(const mrl_attention a, float*
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
-struct Plan { int dp, nt, v_tiles, seg, n_splits; };
+struct Plan { int dp, seg, n_splits, pack; };
 
 int chunk_of(int dtype) { return dtype == MRL_F32 ? El<float>::C : El<__bf16>::C; }
 
@@ -690,16 +673,17 @@ Plan plan_of(const mrl_attention* p, int roles) {
   Plan r;
   const int d = std::max(p->dim_k, p->dim_v);
   r.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128;
-  r.nt = 1;
-  r.v_tiles = 1;
   const int C = chunk_of(p->dtype);
-  const int64_t blocks = std::max<int64_t>(1, p->batch * p->heads * r.v_tiles * roles);
+  const int64_t blocks = std::max<int64_t>(1, p->batch * p->heads * roles);
   const int64_t chunks = cdiv(p->steps, C);
   int64_t splits = std::min<int64_t>(cdiv(2048 / (r.dp / 16), blocks), chunks);
   if (splits < 2) splits = 1;
   const int64_t per = std::max<int64_t>(1, cdiv(chunks, splits));
   r.seg = (int)(per * C);
   r.n_splits = (int)std::max<int64_t>(1, cdiv(chunks, per));
+  // Sequences of one chunk, more of them than the card holds blocks: that many blocks (a multiple of the heads) walk over them.
+  const int64_t resident = std::max<int64_t>(1, 2048 / (r.dp / 16) / roles / p->heads) * p->heads;
+  r.pack = p->steps > 0 && chunks == 1 && p->batch * p->heads >= 2 * resident ? (int)resident : 0;
   return r;
 }
 
@@ -711,27 +695,32 @@ int64_t ws_bytes(const mrl_attention* p, const Plan& pl, int roles) {
   return role_floats(p, pl) * roles * 4 + (int64_t)roles * pl.n_splits * p->batch * p->heads * 4;
 }
 
-template <typename T, int DP, int NT, bool VEC> void launch_as(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
-  const unsigned gx = (unsigned)(a.BH * pl.v_tiles), nth = DP / 16 / NT * 64;
+template <typename T, int DP, bool FULL> void launch_as(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
+  const unsigned nth = DP / 16 * 64;
+  if constexpr (FULL && DP <= 64) {
+    if (pl.pack > 0) {
+      hipLaunchKernelGGL((scan_kernel<T, DP, false, true, true>), dim3(pl.pack, 1, roles), dim3(nth), 0, st, a);
+      return;
+    }
+  }
   if (pl.n_splits > 1) {
-    hipLaunchKernelGGL((scan_kernel<T, DP, NT, true, VEC, false>), dim3(gx, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
+    hipLaunchKernelGGL((scan_kernel<T, DP, true, FULL, false>), dim3(a.BH, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
     const int64_t sz = (int64_t)a.role[0].dq * a.role[0].dv;
     hipLaunchKernelGGL(prefix_kernel, dim3((unsigned)cdiv(sz, 256), a.BH, roles), dim3(256), 0, st, a);
   }
-  if (a.T <= El<T>::C) hipLaunchKernelGGL((scan_kernel<T, DP, NT, false, VEC, true>), dim3(gx, 1, roles), dim3(nth), 0, st, a);
-  else hipLaunchKernelGGL((scan_kernel<T, DP, NT, false, VEC, false>), dim3(gx, pl.n_splits, roles), dim3(nth), 0, st, a);
+  hipLaunchKernelGGL((scan_kernel<T, DP, false, FULL, false>), dim3(a.BH, pl.n_splits, roles), dim3(nth), 0, st, a);
 }
 template <typename T> void launch(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
-  bool vec = true;
-  for (int i = 0; i < roles; ++i) vec = vec && a.role[i].vec;
+  bool full = true;
+  for (int i = 0; i < roles; ++i) full = full && a.role[i].vec && a.role[i].dq == pl.dp && a.role[i].dv == pl.dp;
   auto go = [&](auto v) {
-    constexpr bool VEC = decltype(v)::value;
-    if (pl.dp == 32) launch_as<T, 32, 1, VEC>(a, pl, roles, st);
-    else if (pl.dp == 64) launch_as<T, 64, 1, VEC>(a, pl, roles, st);
-    else if (pl.dp == 96) launch_as<T, 96, 1, VEC>(a, pl, roles, st);
-    else launch_as<T, 128, 1, VEC>(a, pl, roles, st);
+    constexpr bool FULL = decltype(v)::value;
+    if (pl.dp == 32) launch_as<T, 32, FULL>(a, pl, roles, st);
+    else if (pl.dp == 64) launch_as<T, 64, FULL>(a, pl, roles, st);
+    else if (pl.dp == 96) launch_as<T, 96, FULL>(a, pl, roles, st);
+    else launch_as<T, 128, FULL>(a, pl, roles, st);
   };
-  if (vec) go(std::true_type());
+  if (full) go(std::true_type());
   else go(std::false_type());
 }
 int dispatch(const mrl_attention* p, ScanP& a, const Plan& pl, int roles, void* ws, int64_t bytes, void* stream, const char* what) {
@@ -754,7 +743,7 @@ int dispatch(const mrl_attention* p, ScanP& a, const Plan& pl, int roles, void* 
 
 struct Operand { const void* p; const int64_t* s; };
 
-// 16-byte loads: the width is a whole number of units, and so are the address and every stride that is used
+// 16-byte addresses: the first one, and every stride that is used
 bool whole(const Operand& o, int dim, int es, const mrl_attention* p) {
   const int e = 16 / es;
   return dim % e == 0 && ((uintptr_t)o.p & 15) == 0 && (p->batch == 1 || o.s[0] % e == 0) && (p->steps <= 1 || o.s[1] % e == 0) && (p->heads == 1 || o.s[2] % e == 0);
