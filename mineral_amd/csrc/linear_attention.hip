@@ -273,11 +273,8 @@ struct Stage {
       if (row + ROWS * i < n && (FULL || cols > 0)) {          // row < n <= C also keeps the unit inside the tile
         const T* q = p + step * (ROWS * i);
         if constexpr (FULL) w = *reinterpret_cast<const u32x4*>(q);
-        else if (cols >= E || dim >= E) {            // a row's last, cut unit: the 16 bytes that end with the row, moved down
-          const int over = cols < E ? E - cols : 0;
-          __builtin_memcpy(&w, q - over, 16);
-          if (over) w = down(w, over * (int)sizeof(T) * 8);
-        } else {
+        else if (dim >= E) __builtin_memcpy(&w, q - (cols < E ? E - cols : 0), 16);   // a row's last, cut unit: the 16 bytes that end
+        else {                                                                         // with the row, moved down when they are used
           for (int e = 0; e < cols; ++e) {
             if constexpr (sizeof(T) == 4) w[e] = __builtin_bit_cast(unsigned, q[e]);
             else w[e / 2] |= (unsigned)__builtin_bit_cast(unsigned short, q[e]) << (16 * (e & 1));
@@ -294,9 +291,11 @@ struct Stage {
     if (bits) { v[0] = v[0] >> bits | v[1] << (64 - bits); v[1] >>= bits; }
     return __builtin_bit_cast(u32x4, v);
   }
-  __device__ __forceinline__ void store(char* tile, int tid, Peak<T>& peak) const {
+  template <bool FULL> __device__ __forceinline__ void store(char* tile, int cols, int dim, int tid, Peak<T>& peak) {
+    const int over = !FULL && dim >= E && cols > 0 && cols < E ? (E - cols) * (int)sizeof(T) * 8 : 0;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
+      if (!FULL && over) r[i] = down(r[i], over);
       peak.see(r[i]);
       char* q = tile + (tid / UPR + ROWS * i) * PITCH;
       const int cu = tid % UPR;
@@ -430,9 +429,9 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
       plain_n = rm ? 0 : n;
     }
     Peak<T> peak;
-    if constexpr (!STATE) sq.store(lq, tid, peak);
-    sk.store(lk, tid, peak);
-    sv.store(lv, tid, peak);
+    if constexpr (!STATE) sq.template store<FULL>(lq, nq, dq, tid, peak);
+    sk.template store<FULL>(lk, nq, dq, tid, peak);
+    sv.template store<FULL>(lv, nv, dv, tid, peak);
     if (peak.wild()) wild[turn] = 1;
     __syncthreads();
     const bool found = wild[turn] != 0;
@@ -466,7 +465,7 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
 #pragma unroll
       for (int it = 0; it < CT; ++it) {
         if (16 * it >= n) break;
-        asm volatile("" ::: "memory");                   // k is read from LDS again for every 16 rows: kept, it would cost half the waves
+        if constexpr (X::PLANES == 3) asm volatile("" ::: "memory");   // and again for every 16 rows, not kept in registers
         Raw qf[KS];
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] = row_frag<T, SQ::PITCH>(lq, 16 * it + m, s, g);
@@ -491,7 +490,7 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
             if (jt <= it) {
 #pragma unroll
               for (int ks = 0; ks < KS; ++ks) {
-                if (X::PLANES == 3 || ks == 0) asm volatile("" ::: "memory");    // fragments of k are read as they are needed, not all at once
+                if constexpr (X::PLANES == 3) asm volatile("" ::: "memory");   // three planes: fragments are read as they are needed
                 if (32 * ks < dq) X::score(a, row_frag<T, SQ::PITCH>(lk, 16 * jt + m, ks, g), qf[ks]);
               }
 #pragma unroll
@@ -517,7 +516,6 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
       }
     }
     // ---- the state after the chunk
-    asm volatile("" ::: "memory");
     const float dec = n == C ? pC : pw[n];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
@@ -667,8 +665,10 @@ int check_pointers(const mrl_attention* p, const char* what) {
   return MRL_OK;
 }
 
-// How the work is cut: 2048 waves (two a SIMD) keep the card busy, a block has one for every 16 value columns.  With fewer blocks the
-// tokens are split into segments of whole chunks, whose states are computed first, joined, and handed to the second pass.
+// How the work is cut.  A block has one wave for every 16 value columns.  Where there are blocks for every CU and waves for every SIMD,
+// one walks over all its tokens: 272 blocks of 64 x 64, 655 tokens, take 95 us in fp32 and 48 in bf16, split in two 122 and 71.  With
+// fewer the tokens are split into segments of whole chunks, whose states are computed first, joined, and handed to the second pass,
+// 2048 waves in all (two a SIMD): 8 blocks of 128 x 128, 16384 tokens, take 96 us so, 145 with half as many waves and 114 with twice.
 Plan plan_of(const mrl_attention* p, int roles) {
   Plan r;
   const int d = std::max(p->dim_k, p->dim_v);
@@ -676,13 +676,13 @@ Plan plan_of(const mrl_attention* p, int roles) {
   const int C = chunk_of(p->dtype);
   const int64_t blocks = std::max<int64_t>(1, p->batch * p->heads * roles);
   const int64_t chunks = cdiv(p->steps, C);
-  int64_t splits = std::min<int64_t>(cdiv(2048 / (r.dp / 16), blocks), chunks);
-  if (splits < 2) splits = 1;
+  const int waves = r.dp / 16;
+  int64_t splits = blocks >= std::max(256, 1024 / waves) ? 1 : std::max<int64_t>(1, std::min<int64_t>(cdiv(2048 / waves, blocks), chunks));
   const int64_t per = std::max<int64_t>(1, cdiv(chunks, splits));
   r.seg = (int)(per * C);
   r.n_splits = (int)std::max<int64_t>(1, cdiv(chunks, per));
   // Sequences of one chunk, more of them than the card holds blocks: that many blocks (a multiple of the heads) walk over them.
-  const int64_t resident = std::max<int64_t>(1, 2048 / (r.dp / 16) / roles / p->heads) * p->heads;
+  const int64_t resident = std::max<int64_t>(1, 2048 / waves / roles / p->heads) * p->heads;
   r.pack = p->steps > 0 && chunks == 1 && p->batch * p->heads >= 2 * resident ? (int)resident : 0;
   return r;
 }
