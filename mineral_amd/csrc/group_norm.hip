@@ -63,10 +63,18 @@ template <typename T> __device__ __forceinline__ void put_param(void* p, int pdt
   else static_cast<T*>(p)[c] = (T)v;
 }
 
-// sum over the TL lanes of a team (TL a power of two up to 64): every lane gets it
+// sum over the TL lanes of a team (TL a power of two up to 64): every lane gets it.  Up to 16 lanes through the register file's own
+// lane permutations (neighbours, pairs, then the halves of 8 and 16 mirrored, whose lanes hold equal sums by then), not through LDS.
+template <int CTRL> __device__ __forceinline__ float lanes(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
 template <int TL> __device__ __forceinline__ float team_sum(float v) {
-#pragma unroll
-  for (int o = 1; o < TL; o <<= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (TL >= 2) v += lanes<0xb1>(v);
+  if constexpr (TL >= 4) v += lanes<0x4e>(v);
+  if constexpr (TL >= 8) v += lanes<0x141>(v);
+  if constexpr (TL >= 16) v += lanes<0x140>(v);
+  if constexpr (TL >= 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (TL >= 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
 

@@ -617,8 +617,8 @@ int check(const mrl_linear* p, const char* what) {
 }
 
 // Tile edge: 128 where its tiles fill the card, otherwise smaller ones, whose reduction is shared by the block's waves at 32.
-int edge_of(int64_t m, int64_t n) {
-  if (cdiv(m, 256) * cdiv(n, 256) >= 200 && n >= 192) return 256;
+int edge_of(int64_t m, int64_t n, int dtype) {
+  if (cdiv(m, dtype == MRL_F32 ? 128 : 256) * cdiv(n, 256) >= 200 && n >= 192) return 256;
   if (cdiv(m, 128) * cdiv(n, 128) >= 256) return 128;
   if (cdiv(m, 64) * cdiv(n, 64) >= 256) return 64;
   return 32;
@@ -629,13 +629,15 @@ bool direct_ok(const void* base, int64_t ld, int es) { return ((uintptr_t)base &
 
 template <typename T, int LA, int LB> void multiply(MmP& a, int edge, int splits, hipStream_t st) {
   const bool direct = sizeof(T) == 2 && direct_ok(a.a, a.lda, 2) && direct_ok(a.b, a.ldb, 2);
-  if (edge == 256 && (!direct || LB == LAY_K)) edge = 128;
-  a.m_tiles = (int)cdiv(a.M, edge);
+  const bool wide = sizeof(T) == 4 && edge == 256;          // fp32: 128 x 256
+  if (edge == 256 && !wide && (!direct || LB == LAY_K)) edge = 128;
+  a.m_tiles = (int)cdiv(a.M, wide ? 128 : edge);
   a.n_tiles = (int)cdiv(a.N, edge);
   a.blocks = a.m_tiles * a.n_tiles * splits;
   const dim3 grid((unsigned)(cdiv(a.blocks, 8) * 8));
   if constexpr (sizeof(T) == 4) {
-    if (edge >= 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
+    if (wide) hipLaunchKernelGGL((mm_kernel<T, 128, 256, 32, 2, 4, 1, LA, LB, 1, false>), grid, dim3(512), 0, st, a);
+    else if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
     else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
   } else if (direct) {
@@ -660,7 +662,7 @@ struct Plan { int edge_x, edge_w, splits; int64_t r_split; int rows, parts; int6
 Plan plan_of(const mrl_linear* p) {
   Plan r{};
   const int64_t es = p->dtype == MRL_F32 ? 4 : 2;
-  r.edge_x = edge_of(p->rows, p->inputs);
+  r.edge_x = edge_of(p->rows, p->inputs, p->dtype);
   // dW: 128 x 128 tiles where both widths have them; rows split so that about 512 blocks run, in whole steps of 64
   r.edge_w = std::min(p->inputs, p->outputs) >= 192 && std::max(p->inputs, p->outputs) >= 512 && p->rows >= 4096 ? 256 : std::min(p->inputs, p->outputs) >= 96 ? 128 : std::min(p->inputs, p->outputs) >= 48 ? 64 : 32;
   const int64_t tiles = std::max<int64_t>(1, cdiv(p->outputs, r.edge_w) * cdiv(p->inputs, r.edge_w));
@@ -684,7 +686,7 @@ int forward(const mrl_linear* p, const void* x, const void* w, const void* bias,
   MmP a{};
   a.a = x; a.lda = p->x_stride; a.b = w; a.ldb = p->inputs; a.M = (int)p->rows; a.N = p->outputs; a.R = p->inputs; a.r_split = std::max(p->inputs, 1);
   a.y = y; a.bias = bias; a.residual = residual; a.slope = slope; a.act = p->act;
-  multiply<T, LAY_K, LAY_K>(a, edge_of(p->rows, p->outputs), 1, st);
+  multiply<T, LAY_K, LAY_K>(a, edge_of(p->rows, p->outputs, p->dtype), 1, st);
   return MRL_OK;
 }
 

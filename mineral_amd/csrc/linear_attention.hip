@@ -516,6 +516,7 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
       }
     }
     // ---- the state after the chunk
+    if constexpr (X::PLANES == 3) asm volatile("" ::: "memory");
     const float dec = n == C ? pC : pw[n];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
