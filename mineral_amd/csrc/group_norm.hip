@@ -13,6 +13,8 @@
 // order: no atomics.
 #include "memory_common.hip.h"
 
+#include <type_traits>
+
 using namespace mrl::mem;
 
 namespace {
@@ -35,6 +37,34 @@ template <typename T, int V> struct Vec {
 #pragma unroll
       for (int e = 0; e < V; ++e) r[e] = (T)x[e];
       *reinterpret_cast<tv*>(p) = r;
+    }
+  }
+};
+
+// The same at any address, of which `left` elements belong to the row (the others read as zero and are not stored).
+template <typename T, int V> struct Ragged {
+  typedef T tv __attribute__((ext_vector_type(V)));
+  static __device__ __forceinline__ void load(const T* p, int left, float (&x)[V]) {
+    if (left >= V) {
+      tv r;
+      __builtin_memcpy(&r, p, sizeof(r));
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = (float)r[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = e < left ? (float)p[e] : 0.0f;
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, int left, const float (&x)[V]) {
+    if (left >= V) {
+      tv r;
+#pragma unroll
+      for (int e = 0; e < V; ++e) r[e] = (T)x[e];
+      __builtin_memcpy(p, &r, sizeof(r));
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < left) p[e] = (T)x[e];
     }
   }
 };
@@ -80,7 +110,8 @@ template <int TL> __device__ __forceinline__ float team_sum(float v) {
 
 // ---- one pixel per sample --------------------------------------------------------------------------------------------------------
 // Row r = n G + g is Cg contiguous values.  A team of TL lanes, NV vectors per lane, walks the rows team, team + teams, ... of its group.
-template <typename T, int V, int TL, int NV>
+// RAG: Cg is not a number of whole vectors, and rows lie on any address.
+template <typename T, int V, int TL, int NV, bool RAG>
 __global__ __launch_bounds__(256) void token_fwd_kernel(const GnP p) {
   const int lane = threadIdx.x % TL;
   const int team = blockIdx.x * (256 / TL) + threadIdx.x / TL;
@@ -96,10 +127,19 @@ __global__ __launch_bounds__(256) void token_fwd_kernel(const GnP p) {
     in[i] = c < p.Cg;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      w[i][e] = in[i] ? param<T>(p.w, p.pdt, g * p.Cg + c + e, 1.0f) : 0.0f;
-      b[i][e] = in[i] ? param<T>(p.b, p.pdt, g * p.Cg + c + e, 0.0f) : 0.0f;
+      w[i][e] = in[i] && (!RAG || c + e < p.Cg) ? param<T>(p.w, p.pdt, g * p.Cg + c + e, 1.0f) : 0.0f;
+      b[i][e] = in[i] && (!RAG || c + e < p.Cg) ? param<T>(p.b, p.pdt, g * p.Cg + c + e, 0.0f) : 0.0f;
     }
   }
+  auto left = [&](int i) { return p.Cg - (lane + TL * i) * V; };
+  auto read = [&](const T* row, int i, float (&f)[V]) {
+    if constexpr (RAG) Ragged<T, V>::load(row + (lane + TL * i) * V, left(i), f);
+    else Vec<T, V>::load(row + (lane + TL * i) * V, f);
+  };
+  auto write = [&](T* row, int i, const float (&f)[V]) {
+    if constexpr (RAG) Ragged<T, V>::store(row + (lane + TL * i) * V, left(i), f);
+    else Vec<T, V>::store(row + (lane + TL * i) * V, f);
+  };
   for (int64_t r = team; r < rows; r += p.teams) {
     const T* x = static_cast<const T*>(p.x) + r * p.Cg;
     T* y = static_cast<T*>(p.y) + r * p.Cg;
@@ -107,7 +147,7 @@ __global__ __launch_bounds__(256) void token_fwd_kernel(const GnP p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (in[i]) {
-        Vec<T, V>::load(x + (lane + TL * i) * V, v[i]);
+        read(x, i, v[i]);
 #pragma unroll
         for (int e = 0; e < V; ++e) s += v[i][e];
       }
@@ -118,7 +158,7 @@ __global__ __launch_bounds__(256) void token_fwd_kernel(const GnP p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           v[i][e] -= mean;
-          q = __builtin_fmaf(v[i][e], v[i][e], q);
+          if (!RAG || e < left(i)) q = __builtin_fmaf(v[i][e], v[i][e], q);
         }
       }
     const float rstd = 1.0f / sqrtf(team_sum<TL>(q) * inv + p.eps);
@@ -128,7 +168,7 @@ __global__ __launch_bounds__(256) void token_fwd_kernel(const GnP p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[i][e] = __builtin_fmaf(v[i][e] * rstd, w[i][e], b[i][e]);
         act_fwd<V>(p.act, v[i]);
-        Vec<T, V>::store(y + (lane + TL * i) * V, v[i]);
+        write(y, i, v[i]);
       }
     if (p.mean && lane == 0) {
       p.mean[r] = mean;
@@ -138,7 +178,7 @@ __global__ __launch_bounds__(256) void token_fwd_kernel(const GnP p) {
 }
 
 // The teams' parameter sums go to ws as rows [2][C]: row team / G, or one row per block where its teams hold every group equally often.
-template <typename T, int V, int TL, int NV>
+template <typename T, int V, int TL, int NV, bool RAG>
 __global__ __launch_bounds__(256) void token_bwd_kernel(const GnP p) {
   constexpr int TB = 256 / TL;
   __shared__ float red[2][V][256];
@@ -156,11 +196,20 @@ __global__ __launch_bounds__(256) void token_bwd_kernel(const GnP p) {
     in[i] = live && c < p.Cg;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      w[i][e] = in[i] ? param<T>(p.w, p.pdt, g * p.Cg + c + e, 1.0f) : 0.0f;
-      b[i][e] = in[i] ? param<T>(p.b, p.pdt, g * p.Cg + c + e, 0.0f) : 0.0f;
+      w[i][e] = in[i] && (!RAG || c + e < p.Cg) ? param<T>(p.w, p.pdt, g * p.Cg + c + e, 1.0f) : 0.0f;
+      b[i][e] = in[i] && (!RAG || c + e < p.Cg) ? param<T>(p.b, p.pdt, g * p.Cg + c + e, 0.0f) : 0.0f;
       dw[i][e] = db[i][e] = 0.0f;
     }
   }
+  auto left = [&](int i) { return p.Cg - (lane + TL * i) * V; };
+  auto read = [&](const T* row, int i, float (&f)[V]) {
+    if constexpr (RAG) Ragged<T, V>::load(row + (lane + TL * i) * V, left(i), f);
+    else Vec<T, V>::load(row + (lane + TL * i) * V, f);
+  };
+  auto write = [&](T* row, int i, const float (&f)[V]) {
+    if constexpr (RAG) Ragged<T, V>::store(row + (lane + TL * i) * V, left(i), f);
+    else Vec<T, V>::store(row + (lane + TL * i) * V, f);
+  };
   if (live) {
     for (int64_t r = team; r < rows; r += p.teams) {
       const T* x = static_cast<const T*>(p.x) + r * p.Cg;
@@ -171,8 +220,8 @@ __global__ __launch_bounds__(256) void token_bwd_kernel(const GnP p) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (in[i]) {
-          Vec<T, V>::load(x + (lane + TL * i) * V, v[i]);
-          Vec<T, V>::load(dy + (lane + TL * i) * V, d[i]);
+          read(x, i, v[i]);
+          read(dy, i, d[i]);
         }
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -200,7 +249,7 @@ __global__ __launch_bounds__(256) void token_bwd_kernel(const GnP p) {
         if (in[i]) {
 #pragma unroll
           for (int e = 0; e < V; ++e) d[i][e] = rstd * (d[i][e] - m1 - v[i][e] * m2);
-          Vec<T, V>::store(dx + (lane + TL * i) * V, d[i]);
+          write(dx, i, d[i]);
         }
     }
   }
@@ -222,6 +271,7 @@ __global__ __launch_bounds__(256) void token_bwd_kernel(const GnP p) {
       if (lt < p.G && (lane + TL * i) * V < p.Cg) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
+          if (RAG && e >= left(i)) break;
           float a = 0.0f, q = 0.0f;
           for (int k = lt; k < TB; k += p.G) {
             a += red[0][e][k * TL + lane];
@@ -234,6 +284,7 @@ __global__ __launch_bounds__(256) void token_bwd_kernel(const GnP p) {
     } else if (in[i]) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
+        if (RAG && e >= left(i)) break;
         out[c + e] = dw[i][e];
         out[p.C + c + e] = db[i][e];
       }
@@ -375,10 +426,110 @@ __global__ __launch_bounds__(256) void pixel_stats_kernel(const GnP p) {
   }
 }
 
+// Where vectors reach over the border of a group: moments per channel and part -> ws [n][part][2][C] (mean, centred squares).
 template <typename T, int V>
+__global__ __launch_bounds__(256) void pixel_stats_mixed_kernel(const GnP p) {
+  __shared__ float sn[256], sm[V][256], ss[V][256];
+  const Place q = place<V>(p);
+  const T* x = static_cast<const T*>(p.x) + q.n * p.L * p.C + q.c;
+  float n = 0.0f, m[V], s[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) m[e] = s[e] = 0.0f;
+  constexpr int U = 8;
+  if (q.in) {
+    for (int64_t r = q.p0 + q.row; r < q.p1; r += (int64_t)q.rows * U) {
+      float v[U][V], k = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + (int64_t)u * q.rows < q.p1) {
+          Vec<T, V>::load(x + (r + (int64_t)u * q.rows) * p.C, v[u]);
+          k += 1.0f;
+        }
+      const float ik = 1.0f / k, t = n + k, f = k / t, g = n * f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r + (int64_t)u * q.rows < q.p1) a += v[u][e];
+        a *= ik;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r + (int64_t)u * q.rows < q.p1) b = __builtin_fmaf(v[u][e] - a, v[u][e] - a, b);
+        const float d = a - m[e];
+        m[e] = __builtin_fmaf(d, f, m[e]);
+        s[e] += b + d * d * g;
+      }
+      n = t;
+    }
+  }
+  const int t = threadIdx.x;
+  sn[t] = n;
+#pragma unroll
+  for (int e = 0; e < V; ++e) { sm[e][t] = m[e]; ss[e][t] = s[e]; }
+  for (int k = q.rows; k > 1;) {
+    const int h = (k + 1) / 2;
+    __syncthreads();
+    if (q.row < k - h) {
+      const int o = t + h * p.cvs;
+      float n0 = n;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        n0 = n;
+        join_moments(n0, m[e], s[e], sn[o], sm[e][o], ss[e][o]);
+        sm[e][t] = m[e]; ss[e][t] = s[e];
+      }
+      n = n0;
+      sn[t] = n;
+    }
+    k = h;
+  }
+  if (q.row == 0 && q.in) {
+    float* o = p.ws + (q.n * p.splits + q.part) * 2 * p.C + q.c;
+#pragma unroll
+    for (int e = 0; e < V; ++e) { o[e] = m[e]; o[p.C + e] = s[e]; }
+  }
+}
+// One block per (sample, group): the channels' moments of all parts joined -> mean, rstd.
+__global__ __launch_bounds__(1024) void pixel_stats_join_kernel(const GnP p, float* __restrict__ mean, float* __restrict__ rstd) {
+  __shared__ float sn[1024], sm[1024], ss[1024];
+  const int64_t ng = blockIdx.x, sample = ng / p.G;
+  const int g = (int)(ng % p.G), t = threadIdx.x;
+  float n = 0.0f, m = 0.0f, s = 0.0f;
+  for (int k = t; k < p.Cg * p.splits; k += blockDim.x) {
+    const int part = k / p.Cg, c = g * p.Cg + k % p.Cg;
+    const float* o = p.ws + (sample * p.splits + part) * 2 * p.C + c;
+    join_moments(n, m, s, (float)min<int64_t>(p.chunk, p.L - (int64_t)part * p.chunk), o[0], o[p.C]);
+  }
+  sn[t] = n; sm[t] = m; ss[t] = s;
+  for (int h = blockDim.x / 2; h >= 1; h >>= 1) {
+    __syncthreads();
+    if (t < h) {
+      join_moments(n, m, s, sn[t + h], sm[t + h], ss[t + h]);
+      sn[t] = n; sm[t] = m; ss[t] = s;
+    }
+  }
+  if (t == 0) {
+    const float r = 1.0f / sqrtf(s / n + p.eps);
+    mean[ng] = m;
+    rstd[ng] = r;
+    if (p.mean) { p.mean[ng] = m; p.rstd[ng] = r; }
+  }
+}
+
+template <typename T, int V, bool MIXED>
 __global__ __launch_bounds__(256) void pixel_fwd_kernel(const GnP p) {
   __shared__ float sn[256], sm[256], ss[256];
   const Place q = place<V>(p);
+  float mean[MIXED ? V : 1], rstd[MIXED ? V : 1];
+  if constexpr (MIXED) {
+    if (!q.in) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      mean[e] = p.cmean[q.n * p.G + (q.c + e) / p.Cg];
+      rstd[e] = p.crstd[q.n * p.G + (q.c + e) / p.Cg];
+    }
+  } else {
   // the parts' moments of the block's groups: thread t joins parts t / groups, ... of group t % groups, then halves
   const int gpb = p.spg > 1 ? 1 : p.cvs / q.cgv, parts = p.splits * p.spg;
   const int g0 = p.spg > 1 ? q.g : (q.c - q.col * V) / p.Cg;
@@ -402,10 +553,12 @@ __global__ __launch_bounds__(256) void pixel_fwd_kernel(const GnP p) {
   __syncthreads();
   if (!q.in) return;
   const int mine = q.g - g0;
-  const float mean = sm[mine], rstd = 1.0f / sqrtf(ss[mine] / sn[mine] + p.eps);
+  mean[0] = sm[mine];
+  rstd[0] = 1.0f / sqrtf(ss[mine] / sn[mine] + p.eps);
   if (p.mean && q.part == 0 && q.row == 0 && q.j == 0) {
-    p.mean[q.n * p.G + q.g] = mean;
-    p.rstd[q.n * p.G + q.g] = rstd;
+    p.mean[q.n * p.G + q.g] = mean[0];
+    p.rstd[q.n * p.G + q.g] = rstd[0];
+  }
   }
   float w[V], b[V];
 #pragma unroll
@@ -425,7 +578,7 @@ __global__ __launch_bounds__(256) void pixel_fwd_kernel(const GnP p) {
     for (int u = 0; u < U; ++u)
       if (r + (int64_t)u * q.rows < q.p1) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[u][e] = __builtin_fmaf((v[u][e] - mean) * rstd, w[e], b[e]);
+        for (int e = 0; e < V; ++e) v[u][e] = __builtin_fmaf((v[u][e] - mean[MIXED ? e : 0]) * rstd[MIXED ? e : 0], w[e], b[e]);
         act_fwd<V>(p.act, v[u]);
         Vec<T, V>::store(y + (r + (int64_t)u * q.rows) * p.C, v[u]);
       }
@@ -433,7 +586,7 @@ __global__ __launch_bounds__(256) void pixel_fwd_kernel(const GnP p) {
 }
 
 // per channel and part: sum dz xhat, sum dz  ->  ws [n][part][2][C]
-template <typename T, int V>
+template <typename T, int V, bool MIXED>
 __global__ __launch_bounds__(256) void pixel_bwd_sums_kernel(const GnP p) {
   __shared__ float red[2][V][256];
   const Place q = place<V>(p);
@@ -441,8 +594,13 @@ __global__ __launch_bounds__(256) void pixel_bwd_sums_kernel(const GnP p) {
 #pragma unroll
   for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.0f;
   if (q.in) {
-    const int64_t ng = q.n * p.G + q.g;
-    const float mean = p.cmean[ng], rstd = p.crstd[ng];
+    float mean[MIXED ? V : 1], rstd[MIXED ? V : 1];
+#pragma unroll
+    for (int e = 0; e < (MIXED ? V : 1); ++e) {
+      const int64_t ng = q.n * p.G + (MIXED ? (q.c + e) / p.Cg : q.g);
+      mean[e] = p.cmean[ng];
+      rstd[e] = p.crstd[ng];
+    }
     float w[V], b[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -467,7 +625,7 @@ __global__ __launch_bounds__(256) void pixel_bwd_sums_kernel(const GnP p) {
           float z[V];
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            v[u][e] = (v[u][e] - mean) * rstd;
+            v[u][e] = (v[u][e] - mean[MIXED ? e : 0]) * rstd[MIXED ? e : 0];
             z[e] = __builtin_fmaf(v[u][e], w[e], b[e]);
           }
           act_bwd<V>(p.act, z, d[u]);
@@ -551,12 +709,17 @@ __global__ __launch_bounds__(256) void pixel_bwd_join_kernel(const GnP p, float*
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool MIXED>
 __global__ __launch_bounds__(256) void pixel_bwd_dx_kernel(const GnP p, const float* __restrict__ coef) {
   const Place q = place<V>(p);
   if (!q.in) return;
-  const int64_t ng = q.n * p.G + q.g;
-  const float mean = p.cmean[ng], rstd = p.crstd[ng], m1 = coef[2 * ng], m2 = coef[2 * ng + 1];
+  float mean[MIXED ? V : 1], rstd[MIXED ? V : 1], m1[MIXED ? V : 1], m2[MIXED ? V : 1];
+#pragma unroll
+  for (int e = 0; e < (MIXED ? V : 1); ++e) {
+    const int64_t ng = q.n * p.G + (MIXED ? (q.c + e) / p.Cg : q.g);
+    mean[e] = p.cmean[ng]; rstd[e] = p.crstd[ng];
+    m1[e] = coef[2 * ng]; m2[e] = coef[2 * ng + 1];
+  }
   float w[V], b[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -582,12 +745,12 @@ __global__ __launch_bounds__(256) void pixel_bwd_dx_kernel(const GnP p, const fl
         float z[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          v[u][e] = (v[u][e] - mean) * rstd;
+          v[u][e] = (v[u][e] - mean[MIXED ? e : 0]) * rstd[MIXED ? e : 0];
           z[e] = __builtin_fmaf(v[u][e], w[e], b[e]);
         }
         act_bwd<V>(p.act, z, d[u]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) d[u][e] = rstd * (d[u][e] * w[e] - m1 - v[u][e] * m2);
+        for (int e = 0; e < V; ++e) d[u][e] = rstd[MIXED ? e : 0] * (d[u][e] * w[e] - m1[MIXED ? e : 0] - v[u][e] * m2[MIXED ? e : 0]);
         Vec<T, V>::store(dx + (r + (int64_t)u * q.rows) * p.C, d[u]);
       }
   }
@@ -596,7 +759,7 @@ __global__ __launch_bounds__(256) void pixel_bwd_dx_kernel(const GnP p, const fl
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 struct Plan {
   int v;                       // elements of a vector
-  bool tokens;
+  bool tokens, mixed;          // mixed: rows of a token kernel are not whole vectors; vectors of a pixel kernel reach over groups
   int tl, nv, blocks, teams;   // tokens
   int64_t param_rows;          // rows [2][C] that param_sum adds
   int splits, chunk, cvs, slabs, spg;
@@ -614,14 +777,28 @@ int check(const mrl_group_norm* p, const char* what) {
   return MRL_OK;
 }
 
-// vectors of up to 16 bytes that divide a group
 Plan plan_of(const mrl_group_norm* p, bool backward) {
   Plan r{};
-  const int cg = p->channels / p->groups;
-  r.v = p->dtype == MRL_F32 ? 4 : 8;
+  const int cg = p->channels / p->groups, most_v = p->dtype == MRL_F32 ? 4 : 8;
+  // Vectors of up to 16 bytes that divide a group.  Where that leaves single elements, the token kernels take 16-byte vectors and cut the
+  // row's last one (with pairs that costs more than it gives: 38436 rows of 98 take 17.7 us so, 16.4 in pairs).  Where it leaves a
+  // quarter of 16 bytes or less, the pixel kernels let a vector's channels belong to several groups, if the channels divide into wider
+  // ones: 151 x 676 x 184 in 8 groups, fp16, both directions, 171 -> 107 us.
+  r.v = most_v;
   while (cg % r.v) r.v /= 2;
-  const int nv = cg / r.v;
-  r.tokens = p->pixels == 1 && nv <= 64 * 4;
+  r.tokens = p->pixels == 1 && cdiv(cg, r.v == 1 && cg >= most_v ? most_v : r.v) <= 64 * 4;
+  if (r.tokens && r.v == 1 && cg >= most_v) {
+    r.mixed = true;
+    r.v = most_v;
+  } else if (!r.tokens && r.v * 4 <= most_v) {
+    int all = most_v;
+    while (p->channels % all) all /= 2;
+    if (all > r.v) {
+      r.mixed = true;
+      r.v = all;
+    }
+  }
+  const int nv = (int)cdiv(cg, r.v);
   if (r.tokens) {
     r.tl = 1;
     while (r.tl < nv && r.tl < 64) r.tl *= 2;
@@ -638,8 +815,8 @@ Plan plan_of(const mrl_group_norm* p, bool backward) {
     return r;
   }
   // a block takes whole groups; a group of over 256 vectors is cut, and its pieces are joined like parts of the pixels
-  r.spg = (int)cdiv(nv, 256);
-  r.cvs = r.spg > 1 ? 256 : nv * std::max(1, std::min<int>(p->groups, 256 / nv));
+  r.spg = r.mixed ? 1 : (int)cdiv(nv, 256);
+  r.cvs = r.mixed ? std::min(256, p->channels / r.v) : r.spg > 1 ? 256 : nv * std::max(1, std::min<int>(p->groups, 256 / nv));
   r.slabs = r.spg > 1 ? p->groups * r.spg : (int)cdiv(p->channels / r.v, r.cvs);
   const int64_t units = std::max<int64_t>(1, p->batch * r.slabs);
   // about 2048 blocks, and at least eight vectors for each thread
@@ -654,10 +831,11 @@ Plan plan_of(const mrl_group_norm* p, bool backward) {
 
 int64_t part_floats(const mrl_group_norm* p, const Plan& r, bool backward) {
   if (r.tokens) return backward ? r.param_rows * 2 * p->channels : 0;
-  return p->batch * r.splits * (backward ? 2 * (int64_t)p->channels : 3 * (int64_t)p->groups * r.spg);
+  return p->batch * r.splits * (backward || r.mixed ? 2 * (int64_t)p->channels : 3 * (int64_t)p->groups * r.spg);
 }
 int64_t ws_floats(const mrl_group_norm* p, const Plan& r, bool backward) {
   int64_t n = part_floats(p, r, backward);
+  if (!backward && !r.tokens && r.mixed) n += p->batch * p->groups * 2;
   if (backward && !r.tokens) n += p->batch * 2 * (int64_t)p->channels + p->batch * p->groups * 2;
   return n;
 }
@@ -677,7 +855,7 @@ GnP params_of(const mrl_group_norm* p, const Plan& r, void* ws) {
   return a;
 }
 
-template <typename T, int V, typename F> void with_team(const Plan& r, F&& f) {
+template <typename F> void with_team(const Plan& r, F&& f) {
   auto nv = [&](auto tl) {
     constexpr int TL = decltype(tl)::value;
     if (TL < 64 || r.nv == 1) f(tl, std::integral_constant<int, 1>());
@@ -697,30 +875,47 @@ template <typename T, int V, typename F> void with_team(const Plan& r, F&& f) {
   }
 }
 
-template <typename T, int V> void forward(const GnP& a, const Plan& r, hipStream_t st) {
-  if (r.tokens) {
-    with_team<T, V>(r, [&](auto tl, auto nv) {
-      hipLaunchKernelGGL((token_fwd_kernel<T, V, decltype(tl)::value, decltype(nv)::value>), dim3(r.blocks), dim3(256), 0, st, a);
-    });
-    return;
-  }
-  const dim3 grid((unsigned)(a.N * r.splits * r.slabs));
-  hipLaunchKernelGGL((pixel_stats_kernel<T, V>), grid, dim3(256), 0, st, a);
-  hipLaunchKernelGGL((pixel_fwd_kernel<T, V>), grid, dim3(256), 0, st, a);
+template <typename F> void with_flag(bool v, F&& f) {
+  if (v) f(std::true_type());
+  else f(std::false_type());
+}
+// kernels whose vectors are cut or reach over groups have more than one element
+template <typename T, int V> void forward(GnP a, const Plan& r, hipStream_t st, float* stats) {
+  with_flag(r.mixed, [&](auto mixed) {
+    constexpr bool M = decltype(mixed)::value && V > 1;
+    if (r.tokens) {
+      with_team(r, [&](auto tl, auto nv) {
+        hipLaunchKernelGGL((token_fwd_kernel<T, V, decltype(tl)::value, decltype(nv)::value, M>), dim3(r.blocks), dim3(256), 0, st, a);
+      });
+      return;
+    }
+    const dim3 grid((unsigned)(a.N * r.splits * r.slabs));
+    if constexpr (M) {
+      hipLaunchKernelGGL((pixel_stats_mixed_kernel<T, V>), grid, dim3(256), 0, st, a);
+      const unsigned threads = a.Cg * a.splits > 4096 ? 1024 : 256;     // 5120 moments a group: 10 us, 26 by 256 threads; 184: 8 and 5 us
+      hipLaunchKernelGGL(pixel_stats_join_kernel, dim3((unsigned)(a.N * a.G)), dim3(threads), 0, st, a, stats, stats + a.N * a.G);
+      a.cmean = stats;
+      a.crstd = stats + a.N * a.G;
+    } else hipLaunchKernelGGL((pixel_stats_kernel<T, V>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((pixel_fwd_kernel<T, V, M>), grid, dim3(256), 0, st, a);
+  });
 }
 template <typename T, int V> void backward(const GnP& a, const Plan& r, hipStream_t st, float* chan, float* coef) {
   const float* rows = a.ws;
-  if (r.tokens) {
-    with_team<T, V>(r, [&](auto tl, auto nv) {
-      hipLaunchKernelGGL((token_bwd_kernel<T, V, decltype(tl)::value, decltype(nv)::value>), dim3(r.blocks), dim3(256), 0, st, a);
-    });
-  } else {
+  with_flag(r.mixed, [&](auto mixed) {
+    constexpr bool M = decltype(mixed)::value && V > 1;
+    if (r.tokens) {
+      with_team(r, [&](auto tl, auto nv) {
+        hipLaunchKernelGGL((token_bwd_kernel<T, V, decltype(tl)::value, decltype(nv)::value, M>), dim3(r.blocks), dim3(256), 0, st, a);
+      });
+      return;
+    }
     const dim3 grid((unsigned)(a.N * r.splits * r.slabs));
-    hipLaunchKernelGGL((pixel_bwd_sums_kernel<T, V>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((pixel_bwd_sums_kernel<T, V, M>), grid, dim3(256), 0, st, a);
     hipLaunchKernelGGL((pixel_bwd_join_kernel<T>), dim3((unsigned)(a.N * a.G)), dim3(256), 0, st, a, chan, coef);
-    hipLaunchKernelGGL((pixel_bwd_dx_kernel<T, V>), grid, dim3(256), 0, st, a, coef);
+    hipLaunchKernelGGL((pixel_bwd_dx_kernel<T, V, M>), grid, dim3(256), 0, st, a, coef);
     rows = chan;
-  }
+  });
   if (a.dw) hipLaunchKernelGGL((param_sum_kernel<T>), dim3((unsigned)cdiv(2 * (int64_t)a.C, 32)), dim3(1024), 0, st, a, rows, r.param_rows);
 }
 
@@ -747,8 +942,9 @@ int check_grid(const mrl_group_norm* p, const Plan& r, const char* what) {
 // whole vectors on their own size: tensors on odd addresses are served element by element
 int vec_of(const Plan& r, int dtype, std::initializer_list<const void*> ps) {
   const int es = dtype == MRL_F32 ? 4 : 2;
+  const int n = r.tokens && r.mixed ? 1 : r.v;              // cut rows lie on any address anyway
   for (const void* q : ps)
-    if ((uintptr_t)q % (uintptr_t)(r.v * es)) return 0;
+    if ((uintptr_t)q % (uintptr_t)(n * es)) return 0;
   return 1;
 }
 
@@ -774,7 +970,7 @@ extern "C" int mrl_group_norm_act(const mrl_group_norm* p, const void* x, const 
   GnP a = params_of(p, r, workspace);
   a.x = x; a.w = weight; a.b = bias; a.y = y; a.mean = mean; a.rstd = rstd;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  with_type(p->dtype, r.v, [&](auto tag, auto v) { forward<decltype(tag), decltype(v)::value>(a, r, st); });
+  with_type(p->dtype, r.v, [&](auto tag, auto v) { forward<decltype(tag), decltype(v)::value>(a, r, st, a.ws + part_floats(p, r, false)); });
   MEM_CHECK_LAUNCH(what);
   return MRL_OK;
 }

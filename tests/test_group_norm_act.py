@@ -71,7 +71,8 @@ def bounds(x, G, w, b, dy, eps):
 
 
 SHAPES = [((5, 24), 4), ((64, 512), 8), ((3, 7), 7), ((2, 9), 3), ((9, 1), 1), ((33, 130), 2), ((4, 640), 1), ((3, 5000), 2), ((1000, 96), 6), ((70, 48), 48),
-          ((2, 3, 3, 32), 8), ((3, 49, 12), 4), ((2, 100, 70), 10), ((1, 31, 33, 64), 32), ((2, 5, 2100), 1), ((1, 3, 2100), 2), ((2, 500, 6), 2), ((4, 2, 30), 3)]
+          ((2, 3, 3, 32), 8), ((3, 49, 12), 4), ((2, 100, 70), 10), ((1, 31, 33, 64), 32), ((2, 5, 2100), 1), ((1, 3, 2100), 2), ((2, 500, 6), 2), ((4, 2, 30), 3), ((2, 676, 184), 8), ((1, 40, 2144), 32),
+          ((70, 63), 1), ((40, 196), 2), ((9, 11), 1)]
 
 
 @pytest.mark.gpu
