@@ -92,7 +92,7 @@ typedef struct mrl_linear {
 } mrl_linear;
 
 /* slope : [rows][outputs] or NULL: act'(x W^T + bias), what the backward call reads where act is not MRL_ACT_NONE: fp32 beside MRL_F32,
- * otherwise 16 bits (sign, 4 bits of exponent, 11 of mantissa). */
+ * otherwise 16 bits each, in a code of the library's own. */
 int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const void* bias, const void* residual, void* y, void* slope, void* stream);
 
 int64_t mrl_linear_act_backward_workspace_bytes(const mrl_linear* p);

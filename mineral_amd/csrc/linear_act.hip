@@ -202,35 +202,42 @@ template <typename T, int N> __device__ __forceinline__ void store_row(T* p, int
   }
 }
 
-// An activation's slope (magnitude below 2) in 16 bits: sign, 4 bits of exponent, 11 of mantissa, rounded to nearest.  What the
-// backward pass needs of z, in z's room but 2^-12 relative at worst (2^-26 absolute below 2^-14): rounded z or slopes in bf16 or
-// fp16 would add as much error to the gradients as their own rounding.  All ones stand for NaN.
-__device__ __forceinline__ unsigned pack_slope(float s) {
-  const unsigned sign = (__float_as_uint(s) >> 16) & 0x8000u;
-  unsigned a = __float_as_uint(__builtin_fabsf(s) * 0x1p-112f);    // now the exponent fits 4 bits (subnormals included)
-  a = (a + 0x7ffu + ((a >> 12) & 1u)) >> 12;
-  return (__builtin_fabsf(s) < 1.9f ? a : 0x7fffu) | sign;
-}
-__device__ __forceinline__ float unpack_slope(unsigned u) {
-  const float a = __uint_as_float((u & 0x7fffu) << 12) * 0x1p112f;
-  return (u & 0x7fffu) == 0x7fffu ? __builtin_nanf("") : (u & 0x8000u) ? -a : a;
-}
+// An activation's slope (magnitude below 2) in 16 bits: sign, EXP bits of exponent, the others mantissa, rounded to nearest.  What the
+// backward pass needs of z, in z's room: rounded z, or slopes in the type itself, would add as much error to the gradients as their
+// own rounding.  Beside bf16 EXP = 4: off by 2^-12 of the slope (2^-26 below 2^-14); beside fp16 EXP = 3: 2^-13 (2^-20 below 2^-6).
+// All ones stand for NaN.
+template <int EXP> struct Slope16 {
+  static constexpr int SHIFT = 8 + EXP;                                  // bits of an fp32 mantissa that go
+  static constexpr float DOWN = EXP == 4 ? 0x1p-112f : 0x1p-120f, BACK = EXP == 4 ? 0x1p112f : 0x1p120f;
+  static __device__ __forceinline__ unsigned pack(float s) {
+    const unsigned sign = (__float_as_uint(s) >> 16) & 0x8000u;
+    unsigned a = __float_as_uint(__builtin_fabsf(s) * DOWN);            // now the exponent fits (subnormals included)
+    a = (a + (1u << (SHIFT - 1)) - 1u + ((a >> SHIFT) & 1u)) >> SHIFT;
+    return (__builtin_fabsf(s) < 1.9f ? a : 0x7fffu) | sign;
+  }
+  static __device__ __forceinline__ float unpack(unsigned u) {
+    const float a = __uint_as_float((u & 0x7fffu) << SHIFT) * BACK;
+    return (u & 0x7fffu) == 0x7fffu ? __builtin_nanf("") : (u & 0x8000u) ? -a : a;
+  }
+};
+template <typename T> struct SlopeCode { typedef Slope16<4> C; };
+template <> struct SlopeCode<_Float16> { typedef Slope16<3> C; };
 template <typename T> struct SlopeOf { typedef unsigned short S; };
 template <> struct SlopeOf<float> { typedef float S; };
-template <typename S> __device__ __forceinline__ void load_slopes(const S* p, int left, float (&x)[8]) {
+template <typename T, typename S> __device__ __forceinline__ void load_slopes(const S* p, int left, float (&x)[8]) {
   if constexpr (sizeof(S) == 4) load_row<float, 8>(p, left, x);
   else {
     const u32x4 w = load_unit<__bf16>(reinterpret_cast<const __bf16*>(p), left);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = unpack_slope((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+    for (int e = 0; e < 8; ++e) x[e] = SlopeCode<T>::C::unpack((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
   }
 }
-template <typename S> __device__ __forceinline__ void store_slopes(S* p, int left, const float (&x)[8]) {
+template <typename T, typename S> __device__ __forceinline__ void store_slopes(S* p, int left, const float (&x)[8]) {
   if constexpr (sizeof(S) == 4) store_row<float, 8>(p, left, x);
   else {
     u32x4 w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = pack_slope(x[2 * e]) | pack_slope(x[2 * e + 1]) << 16;
+    for (int e = 0; e < 4; ++e) w[e] = SlopeCode<T>::C::pack(x[2 * e]) | SlopeCode<T>::C::pack(x[2 * e + 1]) << 16;
     typedef u32x4 __attribute__((aligned(2))) unit;
     if (left >= 8) __builtin_nontemporal_store(w, reinterpret_cast<unit*>(p));
     else {
@@ -282,7 +289,7 @@ template <typename T, int ACT> __device__ __forceinline__ void finish8(const MmP
     typedef typename SlopeOf<T>::S S;
     float d[8];
     act_slope<8>(ACT, v, d);
-    store_slopes<S>(static_cast<S*>(p.slope) + at, left, d);
+    store_slopes<T>(static_cast<S*>(p.slope) + at, left, d);
   }
   act_fwd<8>(ACT, v);
   if (p.residual) {
@@ -535,7 +542,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* _
       for (int u = 0; u < U; ++u)
         if (m + 8 * u < m1) {
           load_row<T, 8>(dy + (m + 8 * u) * N + c, left, d[u]);
-          if (slope) load_slopes(slope + (m + 8 * u) * N + c, left, g[u]);
+          if (slope) load_slopes<T>(slope + (m + 8 * u) * N + c, left, g[u]);
         }
 #pragma unroll
       for (int u = 0; u < U; ++u)

@@ -2,7 +2,8 @@
 
 Tolerances.  u = 2^-24.  A product of r terms is off by (r + 16) u of the sum of its terms' magnitudes, fp32 operands by 4 u more
 (their six bf16 products drop 2^-23 of each).  Activations and their slopes have slopes of at most 1.13 and are themselves within
-16 u of |z| + 1; beside 16-bit types the backward pass reads the slope off by 2^-12 of itself (2^-26 at least), and rounds dz.  A result is rounded once: eps/2."""
+16 u of |z| + 1; beside bf16 the backward pass reads the slope off by 2^-12 of itself (at least 2^-26), beside fp16 by
+2^-13 (at least 2^-20), and rounds dz.  A result is rounded once: eps/2."""
 
 import pytest
 import torch
@@ -56,7 +57,7 @@ def check(M, K, N, dt, act, seed, bias=True, residual=True, inputs=None):
     extra, h = (4 * U if dt == torch.float32 else 0.0), half_of(dt)
     ze = ((K + 16) * U + extra) * (x.abs() @ w.abs().t() + b.abs())
     close(y, yr.detach(), 1.13 * ze + 16 * U * (z.abs() + 1) + 4 * U * (z.abs() + r.abs()), 'y')
-    se = 0 if act is None else 1.13 * ze + 16 * U * (z.abs() + 1) + (0 if dt == torch.float32 else 2.0 ** -12 * slope.abs() + 2.0 ** -26)     # of the slope
+    se = 0 if act is None else 1.13 * ze + 16 * U * (z.abs() + 1) + {torch.float32: 0, torch.bfloat16: 2.0 ** -12 * slope.abs() + 2.0 ** -26, torch.float16: 2.0 ** -13 * slope.abs() + 2.0 ** -20}[dt]     # of the slope
     dz, dze = (dy * slope).abs(), dy.abs() * se
     dzr = dze + (0 if act is None else h * (dz + dze))                                   # and of the rounded dz
     lims = [dzr @ w.abs() + ((N + 16) * U + extra) * ((dz + dzr) @ w.abs()), dzr.t() @ x.abs() + ((M + 16) * U + extra) * ((dz + dzr).t() @ x.abs()),
