@@ -25,7 +25,9 @@ extern "C" {
  *     S_t = exp(log_decay[h]) * S_{t-1} + k_t v_t^T        (S_{t-1} = 0 where resets[b][t] != 0)
  *     o_t = scale * S_t^T q_t
  * for every batch row b and head h, with S of dim_k x dim_v in fp32.  A reset drops whatever the state held, NaN and infinity
- * included, and no token's output depends on a later token or on an earlier episode.  log_decay <= 0 is meant; -inf keeps nothing.
+ * included, and no token's output depends on a later token or on an earlier episode.  log_decay <= 0 is meant; -inf keeps nothing of a
+ * finite state.  fp32 products are formed from three bf16 terms, exact from magnitudes of 2^-100 on (an infinite value makes NaN of what
+ * it belongs to); the state and all sums are fp32.  batch x heads is below 2^23.
  *   q, k : [batch][steps][heads][dim_k], v : [batch][steps][heads][dim_v] of `dtype`; strides {batch, step, head}
  *   log_decay : [heads] fp32;  resets : [batch][steps] bytes or NULL;  initial_state : [batch][heads][dim_k][dim_v] fp32 or NULL (zero) */
 typedef struct mrl_attention {
@@ -42,10 +44,10 @@ typedef struct mrl_attention {
 /* Bytes of workspace of the forward call (backward = 0) or of the backward call (backward = 1); only the sizes are read. */
 int64_t mrl_linear_attention_workspace_bytes(const mrl_attention* p, int32_t backward);
 
-/* out : [batch][steps][heads][dim_v] of dtype, contiguous; final_state : [batch][heads][dim_k][dim_v] fp32. */
+/* out : [batch][steps][heads][dim_v] of dtype, contiguous, on a 16-byte address; final_state : [batch][heads][dim_k][dim_v] fp32. */
 int mrl_linear_attention(const mrl_attention* p, void* out, float* final_state, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Gradients with respect to q, k, v (contiguous, of dtype) and the initial state (fp32); a NULL output is not computed
+/* Gradients with respect to q, k, v (contiguous, of dtype, on 16-byte addresses) and the initial state (fp32); a NULL output is not computed
  * (d_initial_state comes with dv).
  *   d_out : [batch][steps][heads][dim_v], strides like the inputs;  d_final_state : fp32 or NULL (zero). */
 int mrl_linear_attention_backward(const mrl_attention* p, const void* d_out, const int64_t* d_out_stride_host, const float* d_final_state, void* dq,
@@ -64,7 +66,8 @@ int mrl_linear_attention_step(const mrl_attention* p, float* state, void* out, v
 /* Group norm with an activation on channels-last data [batch][pixels][channels]: one mean and variance (divided by the count) for
  * the pixels x channels/groups values of a sample's group,
  *     y = act((x - mean) / sqrt(var + eps) * weight[c] + bias[c]).
- * x and y of `dtype`, contiguous; weight and bias [channels] of `param_dtype` (dtype or MRL_F32), NULL for one and zero. */
+ * x and y of `dtype`, contiguous; weight and bias [channels] of `param_dtype` (dtype or MRL_F32), NULL for one and zero.
+ * Data on 16-byte addresses fits every width; sums are Welford's and pairwise joins of them, in fp32. */
 typedef struct mrl_group_norm {
   int64_t batch, pixels;
   int32_t channels, groups, dtype, param_dtype, act;
@@ -85,7 +88,7 @@ int mrl_group_norm_act_backward(const mrl_group_norm* p, const void* x, const vo
 /* Linear layer: y = act(x W^T + bias) + residual.
  *   x : [rows][inputs], row stride x_stride; weight : [outputs][inputs]; bias : [outputs] or NULL; residual : [rows][outputs] or NULL;
  *   y : [rows][outputs]; all of `dtype`, contiguous but for x.  16-bit operands multiply as they are and fp32 ones as three exact
- *   bf16 terms (six products, error below an fp32 product's rounding); everything accumulates in fp32 and is rounded once. */
+ *   bf16 terms (six products, error below an fp32 product's rounding, for magnitudes from 2^-100 on; an infinite operand gives NaN); everything accumulates in fp32 and is rounded once. */
 typedef struct mrl_linear {
   int64_t rows, x_stride;
   int32_t inputs, outputs, dtype, act;

@@ -892,7 +892,7 @@ template <typename T, int V> void forward(GnP a, const Plan& r, hipStream_t st, 
     const dim3 grid((unsigned)(a.N * r.splits * r.slabs));
     if constexpr (M) {
       hipLaunchKernelGGL((pixel_stats_mixed_kernel<T, V>), grid, dim3(256), 0, st, a);
-      const unsigned threads = a.Cg * a.splits > 4096 ? 1024 : 256;     // 5120 moments a group: 10 us, 26 by 256 threads; 184: 8 and 5 us
+      const unsigned threads = a.Cg * a.splits > 4096 && a.N * a.G <= 65536 ? 1024 : 256;     // 5120 moments a group: 10 us, 26 by 256 threads; 184: 8 and 5 us
       hipLaunchKernelGGL(pixel_stats_join_kernel, dim3((unsigned)(a.N * a.G)), dim3(threads), 0, st, a, stats, stats + a.N * a.G);
       a.cmean = stats;
       a.crstd = stats + a.N * a.G;
@@ -935,7 +935,9 @@ template <typename F> void with_type(int dtype, int v, F&& f) {
 }
 
 int check_grid(const mrl_group_norm* p, const Plan& r, const char* what) {
-  if (!r.tokens && (p->batch * r.splits * r.slabs >= (int64_t(1) << 31) || p->batch * p->groups >= (int64_t(1) << 31))) MEM_FAIL(MRL_EINVAL, "%s: too many samples", what);
+  // blocks of 256 threads, and a grid has less than 2^32 of them
+  if (!r.tokens && (p->batch * r.splits * r.slabs >= (int64_t(1) << 24) || p->batch * p->groups >= (int64_t(1) << 24)))
+    MEM_FAIL(MRL_EINVAL, "%s: %lld samples of %d groups (below 2^24 together)", what, (long long)p->batch, p->groups);
   return MRL_OK;
 }
 

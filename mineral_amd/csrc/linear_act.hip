@@ -523,10 +523,11 @@ __global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
   WE::run(p, t, ep, acc, wave_m, wave_n, lane, res);
 }
 
-// dz = dy slope, and the sums of its columns over this block's rows -> part [blocks in y][N].  32 units of 8 columns x 8 rows a block.
+// dz = dy slope, and the sums of its columns over this block's rows -> part [blocks in y][N], or db where one block has all rows (a
+// launch less for small batches).  32 units of 8 columns x 8 rows a block.
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* __restrict__ slope, const T* __restrict__ dy, T* __restrict__ dz, float* __restrict__ part,
-                                                 int64_t M, int N, int rows) {
+                                                 T* __restrict__ db, int64_t M, int N, int rows) {
   __shared__ float red[8][32 * 8 + 1];
   const int cu = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + cu) * 8, left = N - c;
@@ -557,7 +558,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* _
         }
     }
   }
-  if (!part) return;
+  if (!part && !db) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) red[rl][cu * 8 + e] = s[e];
   __syncthreads();
@@ -566,7 +567,8 @@ __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* _
     float a = 0.0f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) a += red[k][threadIdx.x];
-    part[(int64_t)blockIdx.y * N + col] = a;
+    if (db) db[col] = (T)a;
+    else part[(int64_t)blockIdx.y * N + col] = a;
   }
 }
 
@@ -619,7 +621,8 @@ int check(const mrl_linear* p, const char* what) {
   if (p->rows < 0 || p->inputs < 0 || p->outputs < 0) MEM_FAIL(MRL_EINVAL, "%s: rows %lld, inputs %d, outputs %d", what, (long long)p->rows, p->inputs, p->outputs);
   if (p->rows > (int64_t(1) << 30) || p->inputs > (1 << 24) || p->outputs > (1 << 24)) MEM_FAIL(MRL_EINVAL, "%s: sizes beyond 2^30 rows or 2^24 columns", what);
   if (p->rows > 1 && p->x_stride < p->inputs) MEM_FAIL(MRL_EINVAL, "%s: x_stride %lld below %d inputs", what, (long long)p->x_stride, p->inputs);
-  if (cdiv(p->rows, 32) * cdiv(std::max(p->inputs, p->outputs), 32) >= (int64_t(1) << 30)) MEM_FAIL(MRL_EINVAL, "%s: too many tiles", what);
+  // tiles of at least 128 x 128 where there are many, 256 threads each, and a grid has less than 2^32 of them
+  if (cdiv(std::max<int64_t>(p->rows, p->inputs), 128) * cdiv(std::max(p->inputs, p->outputs), 128) >= (int64_t(1) << 23)) MEM_FAIL(MRL_EINVAL, "%s: %lld rows, %d inputs, %d outputs: over 2^23 tiles", what, (long long)p->rows, p->inputs, p->outputs);
   return MRL_OK;
 }
 
@@ -676,9 +679,9 @@ Plan plan_of(const mrl_linear* p) {
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(r.edge_w == 256 ? 256 : 512, tiles), cdiv(p->rows, 256)));
   r.r_split = std::max<int64_t>(64, cdiv(cdiv(p->rows, splits), 64) * 64);
   r.splits = (int)std::max<int64_t>(1, cdiv(p->rows, r.r_split));
-  // dz: blocks of 256 columns, about 2048 of them
+  // dz: blocks of 256 columns, about 2048 of them; one alone where it has all rows in flight at once
   const int64_t cols = std::max<int64_t>(1, cdiv(p->outputs, 256));
-  r.rows = (int)std::max<int64_t>(8, cdiv(cdiv(p->rows * cols, 2048), 8) * 8);
+  r.rows = p->rows <= 32 ? 32 : (int)std::max<int64_t>(8, cdiv(cdiv(p->rows * cols, 2048), 8) * 8);
   r.parts = (int)std::max<int64_t>(1, cdiv(p->rows, r.rows));
   auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
   r.dz = p->act == MRL_ACT_NONE ? 0 : up(p->rows * p->outputs * es);
@@ -703,11 +706,12 @@ int backward(const mrl_linear* p, const void* x, const void* w, const void* slop
   T* dz = reinterpret_cast<T*>(ws);
   float* part = reinterpret_cast<float*>(ws + r.dz);
   float* slab = reinterpret_cast<float*>(ws + r.dz + r.part);
-  const bool act = p->act != MRL_ACT_NONE;
+  const bool act = p->act != MRL_ACT_NONE, whole = p->rows > 0 && r.parts == 1;
   if (p->rows > 0 && (db || (act && (dx || dw))))
     hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)cdiv(p->outputs, 256), r.parts), dim3(256), 0, st,
-                       act ? static_cast<const typename SlopeOf<T>::S*>(slope) : nullptr, static_cast<const T*>(dy), dz, db ? part : nullptr, p->rows, p->outputs, r.rows);
-  if (db) hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)cdiv(p->outputs, 32)), dim3(1024), 0, st, part, p->rows > 0 ? r.parts : 0, p->outputs, static_cast<T*>(db));
+                       act ? static_cast<const typename SlopeOf<T>::S*>(slope) : nullptr, static_cast<const T*>(dy), dz, db && !whole ? part : nullptr,
+                       whole ? static_cast<T*>(db) : nullptr, p->rows, p->outputs, r.rows);
+  if (db && !whole) hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)cdiv(p->outputs, 32)), dim3(1024), 0, st, part, p->rows > 0 ? r.parts : 0, p->outputs, static_cast<T*>(db));
   const void* d = act ? static_cast<const void*>(dz) : dy;
   if (dx && p->rows > 0 && p->inputs > 0) {
     MmP a{};

@@ -227,7 +227,7 @@ template <> struct Peak<float> {
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = max(m, w[e] & 0x7fffffffu);
   }
-  __device__ __forceinline__ bool wild() const { return m >= 0x7f800000u; }
+  __device__ __forceinline__ bool wild() const { return m >= 0x7f7f8000u; }   // infinite already as a bf16 term
 };
 template <unsigned short INF> struct Peak16 {
   u16x2 m = {0, 0};
@@ -655,8 +655,16 @@ int check(const mrl_attention* p, const char* what) {
   if (p->dim_k < 1 || p->dim_k > MRL_ATTENTION_MAX_DIM || p->dim_v < 1 || p->dim_v > MRL_ATTENTION_MAX_DIM)
     MEM_FAIL(MRL_EINVAL, "%s: dim_k %d, dim_v %d (1..%d each)", what, p->dim_k, p->dim_v, MRL_ATTENTION_MAX_DIM);
   if (p->steps >= (int64_t(1) << 30)) MEM_FAIL(MRL_EINVAL, "%s: %lld steps", what, (long long)p->steps);
-  if (p->batch > (int64_t(1) << 30) / p->heads) MEM_FAIL(MRL_EINVAL, "%s: %lld batch rows x %d heads", what, (long long)p->batch, p->heads);
+  // one block each, and a grid has less than 2^32 threads: 256 of them stepping, up to 512 of a wide scan
+  if (p->batch >= (int64_t(1) << 23) / p->heads) MEM_FAIL(MRL_EINVAL, "%s: %lld batch rows x %d heads (below 2^23)", what, (long long)p->batch, p->heads);
   return MRL_OK;
+}
+
+// outputs are stored in units of up to 16 bytes
+bool on_units(std::initializer_list<const void*> ps) {
+  for (const void* q : ps)
+    if ((uintptr_t)q & 15) return false;
+  return true;
 }
 
 int check_pointers(const mrl_attention* p, const char* what) {
@@ -732,7 +740,10 @@ int dispatch(const mrl_attention* p, ScanP& a, const Plan& pl, int roles, void* 
   a.T = (int)p->steps; a.seg = pl.seg; a.n_splits = pl.n_splits; a.H = p->heads;
   a.BH = (int)(p->batch * p->heads);
   a.ws = static_cast<float*>(ws);
-  for (int i = 0; i < roles; ++i) a.role[i].ws = role_floats(p, pl) * i;
+  for (int i = 0; i < roles; ++i) {
+    a.role[i].ws = role_floats(p, pl) * i;
+    a.role[i].vec = a.role[i].vec && on_units({a.role[i].s0});
+  }
   a.flags = reinterpret_cast<int*>(a.ws + role_floats(p, pl) * roles);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p->dtype == MRL_F32) launch<float>(a, pl, roles, st);
@@ -783,6 +794,7 @@ extern "C" int mrl_linear_attention(const mrl_attention* p, void* out, float* fi
   if (rc || (rc = check_pointers(p, what))) return rc;
   if (p->batch == 0) return MRL_OK;
   if (!final_state || (p->steps > 0 && !out)) MEM_FAIL(MRL_EINVAL, "%s: null output", what);
+  if (!on_units({out})) MEM_FAIL(MRL_EINVAL, "%s: out is not aligned to 16 bytes", what);
   ScanP a;
   Role& r = a.role[0];
   set_role(r, p, false, {p->q, p->q_stride}, {p->k, p->k_stride}, {p->v, p->v_stride}, p->dim_k, p->dim_v, out);
@@ -800,6 +812,7 @@ extern "C" int mrl_linear_attention_backward(const mrl_attention* p, const void*
   if (p->batch == 0) return MRL_OK;
   if (p->steps > 0 && (!d_out || !d_out_stride_host)) MEM_FAIL(MRL_EINVAL, "%s: null d_out", what);
   if (p->steps > 0 && d_initial_state && !dv) MEM_FAIL(MRL_EINVAL, "%s: d_initial_state comes with dv", what);
+  if (!on_units({dq, dk, dv})) MEM_FAIL(MRL_EINVAL, "%s: dq, dk and dv have to be aligned to 16 bytes", what);
   static const int64_t none[3] = {0, 0, 0};
   const Operand q{p->q, p->q_stride}, k{p->k, p->k_stride}, v{p->v, p->v_stride}, d{d_out, d_out_stride_host ? d_out_stride_host : none};
   const int K = p->dim_k, V = p->dim_v;

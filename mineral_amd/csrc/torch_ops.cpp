@@ -206,13 +206,10 @@ Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
   const Attention d(what, q, k, v, l, of(r), state, scale, true);
   if (q.is_cpu()) no_cpu(what);
   c10::DeviceGuard guard(q.device());
+  state.unsafeGetTensorImpl()->bump_version();                            // written below torch's own bookkeeping
   Tensor out = new_like(v, v.sizes());
   check(mrl_linear_attention_step(&d.a, static_cast<float*>(mp(state)), mp(out), stream_of(q)), what);
   return out;
-}
-Tensor linear_attention_step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
-  state.unsafeGetTensorImpl()->bump_version();                            // written below torch's own bookkeeping
-  return linear_attention_step(q, k, v, l, state, r, scale);
 }
 
 // ---- activations -------------------------------------------------------------------------------------------------------------------
@@ -417,7 +414,7 @@ TORCH_LIBRARY_IMPL(mineral, CUDA, m) {
 }
 TORCH_LIBRARY_IMPL(mineral, AutogradCUDA, m) {
   m.impl("linear_attention", linear_attention_autograd);
-  m.impl("linear_attention_step", linear_attention_step_autograd);
+  m.impl("linear_attention_step", linear_attention_step);
   m.impl("group_norm_act", group_norm_act_autograd);
   m.impl("linear_act", linear_act_autograd);
 }

@@ -252,3 +252,5 @@ def test_refusals():
     for bad in (_hip.GroupNorm(4, 1, 8, 3, 0, 0, 0, 1e-5), _hip.GroupNorm(4, 1, 8, 2, 3, 0, 0, 1e-5), _hip.GroupNorm(4, 1, 8, 2, 1, 2, 0, 1e-5),
                 _hip.GroupNorm(4, 1, 8, 2, 0, 0, 9, 1e-5), _hip.GroupNorm(-1, 1, 8, 2, 0, 0, 0, 1e-5)):
         assert L.mrl_group_norm_act_workspace_bytes(bad, 0) == -1
+    many = _hip.GroupNorm(1 << 24, 2, 8, 2, 0, 0, 0, 1e-5)
+    assert L.mrl_group_norm_act(many, 16, None, None, 16, None, None, 16, 1 << 40, None) == -1 and b'2^24' in L.mrl_last_error()

@@ -246,5 +246,5 @@ def test_refusals():
     assert L.mrl_linear_act_backward(a, 16, 16, None, 16, 16, 16, 16, 16, 1 << 30, None) == -1
     a.x_stride = 3
     assert L.mrl_linear_act(a, 16, 16, None, None, 16, None, None) == -1 and b'x_stride' in L.mrl_last_error()
-    for bad in (_hip.Linear(4, 8, 8, 6, 3, 0), _hip.Linear(4, 8, 8, 6, 0, 6), _hip.Linear(-1, 8, 8, 6, 0, 0), _hip.Linear(4, 1 << 25, 1 << 25, 6, 0, 0)):
+    for bad in (_hip.Linear(4, 8, 8, 6, 3, 0), _hip.Linear(4, 8, 8, 6, 0, 6), _hip.Linear(-1, 8, 8, 6, 0, 0), _hip.Linear(4, 1 << 25, 1 << 25, 6, 0, 0), _hip.Linear(1 << 30, 8, 8, 256, 0, 0)):
         assert L.mrl_linear_act_backward_workspace_bytes(bad) == -1

@@ -350,6 +350,13 @@ def test_refusals_on_the_device():
         M.linear_attention(q.requires_grad_(True), k, v, l.clone().requires_grad_(True), r, s, 1.0)
     with pytest.raises(NotImplementedError, match='no gradient'):
         M.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], l, s, None, 1.0)
+    # what a step overwrites is not what an earlier call's gradient reads
+    for mode in (torch.no_grad, torch.inference_mode):
+        out, _ = M.linear_attention(q, k, v, l, r, s, 1.0)
+        with mode():
+            M.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], l, s, None, 1.0)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            out.sum().backward()
     q = q.detach()
     with pytest.raises(ValueError, match='in place'):
         M.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], l, s.transpose(2, 3), None, 1.0)
@@ -386,13 +393,15 @@ def test_refusals():
         return _hip.Attention(B, T, H, K, V, dtype, 16, 16, 16, i3(T * H * K, H * K, K), i3(T * H * K, H * K, K), i3(T * H * V, H * V, V), 16, None, None, 1.0)
     a = desc()
     assert L.mrl_linear_attention_workspace_bytes(a, 0) == 0
-    for bad in (desc(K=129), desc(V=0), desc(H=0), desc(T=-1), desc(T=1 << 30), desc(B=1 << 30), desc(dtype=7)):
+    for bad in (desc(K=129), desc(V=0), desc(H=0), desc(T=-1), desc(T=1 << 30), desc(B=1 << 30), desc(B=1 << 22), desc(dtype=7)):
         assert L.mrl_linear_attention_workspace_bytes(bad, 0) == -1
     assert L.mrl_linear_attention(a, None, None, None, 0, None) == -1 and b'null output' in L.mrl_last_error()
     assert L.mrl_linear_attention(None, None, None, None, 0, None) == -1
     assert L.mrl_linear_attention_step(a, None, None, None) == -1 and b'steps' in L.mrl_last_error()
     assert L.mrl_linear_attention_backward(a, None, None, None, None, None, None, None, None, 0, None) == -1
     assert L.mrl_linear_attention_backward(a, 16, i3(0, 0, 0), None, 16, 16, None, 16, None, 0, None) == -1 and b'd_initial_state' in L.mrl_last_error()
+    assert L.mrl_linear_attention(a, 8, 16, None, 0, None) == -1 and b'aligned' in L.mrl_last_error()
+    assert L.mrl_linear_attention_backward(a, 16, i3(0, 0, 0), None, 16, 8, 16, None, None, 0, None) == -1 and b'aligned' in L.mrl_last_error()
     long = desc(T=4096)
     assert L.mrl_linear_attention_workspace_bytes(long, 0) > 0
     assert L.mrl_linear_attention(long, 16, 16, None, 0, None) == -2 and b'workspace' in L.mrl_last_error()
