@@ -604,11 +604,18 @@ __global__ __launch_bounds__(256) void slab_sum_kernel(const float* __restrict__
   if (i >= n) return;
   const int left = (int)min<int64_t>(4, n - i);
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < splits; ++k) {
-    float v[4];
-    load_row<float, 4>(slab + k * n + i, left, v);
+  constexpr int U = 4;                                      // slabs in flight
+  for (int k = 0; k < splits; k += U) {
+    float v[U][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] += v[e];
+    for (int u = 0; u < U; ++u)
+      if (k + u < splits) load_row<float, 4>(slab + (k + u) * n + i, left, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u < splits) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[u][e];
+      }
   }
   store_row<T, 4>(out + i, left, s);
 }
@@ -626,7 +633,9 @@ int check(const mrl_linear* p, const char* what) {
   return MRL_OK;
 }
 
-// Tile edge: 128 where its tiles fill the card, otherwise smaller ones, whose reduction is shared by the block's waves at 32.
+// Tile edge: the largest whose tiles fill the card; at 32 the block's waves share the reduction.  Measured, at the rule's edge and at
+// its neighbours: dx of 32768 x 2048 -> 512, bf16: 256: 70 us, 128: 82, 64: 113.  Forward 4099 x 333 -> 777, fp16: 64: 18 us, 128: 21,
+// 32: 25.  64 x 512 -> 512, bf16: 32: 4.9 us, 64: 5.8.  fp32 32768 x 256 -> 512: 256 (128 x 256): 63 us, 128: 66, 64: 72.
 int edge_of(int64_t m, int64_t n, int dtype) {
   if (cdiv(m, dtype == MRL_F32 ? 128 : 256) * cdiv(n, 256) >= 200 && n >= 192) return 256;
   if (cdiv(m, 128) * cdiv(n, 128) >= 256) return 128;
@@ -640,7 +649,10 @@ bool direct_ok(const void* base, int64_t ld, int es) { return ((uintptr_t)base &
 template <typename T, int LA, int LB> void multiply(MmP& a, int edge, int splits, hipStream_t st) {
   const bool direct = sizeof(T) == 2 && direct_ok(a.a, a.lda, 2) && direct_ok(a.b, a.ldb, 2);
   const bool wide = sizeof(T) == 4 && edge == 256;          // fp32: 128 x 256
-  if (edge == 256 && !wide && (!direct || LB == LAY_K)) edge = 128;
+  // 256 x 256 forward: only over long reductions with little to load and store besides, as its two blocks of accumulators leave no
+  // registers for that (16384 x 2048 -> 2048, SiLU: 143 us, 128: 171; with residual and slope 203 and 187).
+  const bool lean = LB == LAY_R || (!a.residual && !a.slope && a.R >= 1024);
+  if (edge == 256 && !wide && !(direct && lean)) edge = 128;
   a.m_tiles = (int)cdiv(a.M, wide ? 128 : edge);
   a.n_tiles = (int)cdiv(a.N, edge);
   a.blocks = a.m_tiles * a.n_tiles * splits;
@@ -651,13 +663,8 @@ template <typename T, int LA, int LB> void multiply(MmP& a, int edge, int splits
     else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
   } else if (direct) {
-    if constexpr (LB == LAY_R) {
-      if (edge == 256) {
-        hipLaunchKernelGGL((mm_kernel<T, 256, 256, 32, 2, 4, 1, LA, LB, 4, true>), grid, dim3(512), 0, st, a);
-        return;
-      }
-    }
-    if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 4, true>), grid, dim3(256), 0, st, a);
+    if (edge == 256) hipLaunchKernelGGL((mm_kernel<T, 256, 256, 32, 2, 4, 1, LA, LB, 4, true>), grid, dim3(512), 0, st, a);
+    else if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 4, true>), grid, dim3(256), 0, st, a);
     else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 64, 2, 2, 1, LA, LB, 4, true>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 8, true>), grid, dim3(256), 0, st, a);
   } else {
@@ -673,10 +680,13 @@ Plan plan_of(const mrl_linear* p) {
   Plan r{};
   const int64_t es = p->dtype == MRL_F32 ? 4 : 2;
   r.edge_x = edge_of(p->rows, p->inputs, p->dtype);
-  // dW: 128 x 128 tiles where both widths have them; rows split so that about 512 blocks run, in whole steps of 64
-  r.edge_w = std::min(p->inputs, p->outputs) >= 192 && std::max(p->inputs, p->outputs) >= 512 && p->rows >= 4096 ? 256 : std::min(p->inputs, p->outputs) >= 96 ? 128 : std::min(p->inputs, p->outputs) >= 48 ? 64 : 32;
-  const int64_t tiles = std::max<int64_t>(1, cdiv(p->outputs, r.edge_w) * cdiv(p->inputs, r.edge_w));
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(r.edge_w == 256 ? 256 : 512, tiles), cdiv(p->rows, 256)));
+  // dW: the largest edge of which there are 64 tiles (128 at 256), the rows split until 512 blocks (256 of the large ones) run, each
+  // with at least 1024 rows (512 at 128): more splits cost more in their sums than they win.  8192 x 8192 over 8192 rows, bf16: 256:
+  // 1.01 ms, 128: 1.39.  2048 x 512 over 32768: 128: 82 us, 256: 92, 64: 104.  512 x 512 over 4096: 64: 12 us, 128: 20.
+  auto tiles_of = [&](int edge) { return std::max<int64_t>(1, cdiv(p->outputs, edge) * cdiv(p->inputs, edge)); };
+  r.edge_w = p->dtype != MRL_F32 && tiles_of(256) >= 128 ? 256 : tiles_of(128) >= 64 ? 128 : std::min(p->inputs, p->outputs) >= 48 ? 64 : 32;
+  const int64_t tiles = tiles_of(r.edge_w);
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(r.edge_w == 256 ? 256 : 512, tiles), p->rows / (r.edge_w >= 128 ? 512 : 1024)));
   r.r_split = std::max<int64_t>(64, cdiv(cdiv(p->rows, splits), 64) * 64);
   r.splits = (int)std::max<int64_t>(1, cdiv(p->rows, r.r_split));
   // dz: blocks of 256 columns, about 2048 of them; one alone where it has all rows in flight at once

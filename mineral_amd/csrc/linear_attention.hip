@@ -314,7 +314,8 @@ struct Stage {
 };
 
 // DP: both widths padded; STATE: only the segment's own contribution to the state; FULL: both widths are DP and
-// all rows lie on 16-byte addresses; PACK: sequences of one chunk, several to a block, the next one's loads under way during the present one's products
+// all rows lie on 16-byte addresses; PACK: sequences of one chunk, several to a block, the next one's loads under way during the
+// present one's products
 template <typename T, int DP, bool STATE, bool FULL, bool PACK>
 __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
   typedef El<T> X;
@@ -675,9 +676,9 @@ int check_pointers(const mrl_attention* p, const char* what) {
 }
 
 // How the work is cut.  A block has one wave for every 16 value columns.  Where there are blocks for every CU and waves for every SIMD,
-// one walks over all its tokens: 272 blocks of 64 x 64, 655 tokens, take 95 us in fp32 and 48 in bf16, split in two 122 and 71.  With
+// one walks over all its tokens: 272 blocks of 64 x 64, 655 tokens, take 88 us in fp32 and 47 in bf16, split in two 115 and 69.  With
 // fewer the tokens are split into segments of whole chunks, whose states are computed first, joined, and handed to the second pass,
-// 2048 waves in all (two a SIMD): 8 blocks of 128 x 128, 16384 tokens, take 96 us so, 145 with half as many waves and 114 with twice.
+// 2048 waves in all (two a SIMD): 8 blocks of 128 x 128, 16384 tokens, bf16, take 86 us so, 134 with half as many waves and 102 with twice.
 Plan plan_of(const mrl_attention* p, int roles) {
   Plan r;
   const int d = std::max(p->dim_k, p->dim_v);
@@ -690,9 +691,11 @@ Plan plan_of(const mrl_attention* p, int roles) {
   const int64_t per = std::max<int64_t>(1, cdiv(chunks, splits));
   r.seg = (int)(per * C);
   r.n_splits = (int)std::max<int64_t>(1, cdiv(chunks, per));
-  // Sequences of one chunk, more of them than the card holds blocks: that many blocks (a multiple of the heads) walk over them.
+  // Gradients of sequences of one chunk, more of them than the card holds blocks: that many blocks (a multiple of the heads) walk over
+  // them, with the next one's loads under way.  65536 sequences of 32 x 64: bf16 1218 us so and 1323 with a block each, fp32 1832 and
+  // 1918.  The forward pass (fp32 747 and 737) and narrow heads (32 x 32, 16 tokens, fp32: 601 and 488) keep a block each.
   const int64_t resident = std::max<int64_t>(1, 2048 / waves / roles / p->heads) * p->heads;
-  r.pack = p->steps > 0 && chunks == 1 && p->batch * p->heads >= 2 * resident ? (int)resident : 0;
+  r.pack = roles > 1 && r.dp == 64 && p->steps > 0 && chunks == 1 && p->batch * p->heads >= 2 * resident ? (int)resident : 0;
   return r;
 }
 
@@ -706,7 +709,7 @@ int64_t ws_bytes(const mrl_attention* p, const Plan& pl, int roles) {
 
 template <typename T, int DP, bool FULL> void launch_as(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
   const unsigned nth = DP / 16 * 64;
-  if constexpr (FULL && DP <= 64) {
+  if constexpr (FULL && DP == 64) {
     if (pl.pack > 0) {
       hipLaunchKernelGGL((scan_kernel<T, DP, false, true, true>), dim3(pl.pack, 1, roles), dim3(nth), 0, st, a);
       return;
