@@ -8,6 +8,9 @@ calling an operator with CPU tensors fails in the dispatcher instead of falling 
     import mineral_amd.ops
     torch.ops.mineral.gae_finish(rewards_tn, values_tn, dones_tn, neglogp_tn, last_values, 0.99, 0.95, ...)
 
+The operators of a sequence memory (linear_attention, linear_attention_step, group_norm_act, linear_act) are differentiable and
+registered by memory_ops, which this module imports.
+
 Network description for the operators that run the towers: `net_i` = [obs_dim, act_dim, dist_type, tower_kind, fixed_sigma,
 units...] (dist_type 0 normal / 1 dreamerv3_normal; tower_kind 0 LayerNorm+SiLU / 1 ELU / 2 LayerNorm+ELU) and `net_f` = [minstd, maxstd, ln_eps].
 """
