@@ -8,9 +8,9 @@
 // through LDS once and then works on rows: bias, activation and its slope, residual and stores in 16-byte units.
 // fp32 operands are split exactly into three bf16 terms on their way to LDS and multiply in six products, smallest first.
 // dW sums over all rows: they are split over blocks whose partial sums are added in a fixed order.
-// Bound: 32768 rows, 512 -> 2048, bf16, SiLU, residual: forward 181 us (435 MB to move and 69 GFLOP; the epilogue's loads and stores
+// Bound: 32768 rows, 512 -> 2048, bf16, SiLU, residual: forward 165 us (435 MB to move and 69 GFLOP; the epilogue's loads and stores
 // beside products of 16 steps only), dz 86 us (403 MB, 4.7 TB/s), dx 83 us (828 TFLOP/s), dW 95 + 7 us (723 TFLOP/s); plain products
-// of this shape by the library run at 759.  8192^3: dW 1.07 PFLOP/s.  fp32, 512 -> 256: 57 us, 6 x 150 TFLOP/s of bf16 products.
+// of this shape by the library run at 759.  8192^3: dW 1.07 PFLOP/s.  fp32, 512 -> 256, ELU: 53 us, 6 x 161 TFLOP/s of bf16 products.
 #include "memory_common.hip.h"
 
 using namespace mrl::mem;
@@ -286,7 +286,7 @@ template <typename T> __device__ __forceinline__ void stream_row(T* p, int left,
   } else store_row<T, 8>(p, left, x);
 }
 
-template <typename T, int ACT> __device__ __forceinline__ void finish8(const MmP& p, int64_t at, int left, float (&v)[8], const float (&bias)[8], const T (&res)[8]) {
+template <typename T, int ACT, bool RES> __device__ __forceinline__ void finish8(const MmP& p, int64_t at, int left, float (&v)[8], const float (&bias)[8], const T (&res)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
   if (ACT != MRL_ACT_NONE && p.slope) {
@@ -296,7 +296,7 @@ template <typename T, int ACT> __device__ __forceinline__ void finish8(const MmP
     store_slopes<T>(static_cast<S*>(p.slope) + at, left, d);
   }
   act_fwd<8>(ACT, v);
-  if (p.residual) {
+  if constexpr (RES) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += (float)res[e];
   }
@@ -304,11 +304,12 @@ template <typename T, int ACT> __device__ __forceinline__ void finish8(const MmP
 }
 
 // The epilogue of a wave's TM x TN accumulators, by itself: 32 rows at a time go through its own piece of LDS and leave in units of 8
-// columns, whole cache lines of a row.  The residuals are on their way since the last step.
-template <typename T, int TM, int TN, bool PLAIN> struct WaveEpilogue {
+// columns, whole cache lines of a row.  The residuals (RES: there are any; without, the kernel is smaller by their registers) are on
+// their way since the last step.
+template <typename T, int TM, int TN, bool PLAIN, bool RES> struct WaveEpilogue {
   static constexpr int W = TN * 32, EP = W + 4, BYTES = 32 * EP * 4, UPR = W / 8, UNITS = 32 * UPR / 64;
   typedef T row8[8];
-  static constexpr int AHEAD = TM < 2 ? TM : 2;             // 32-row pieces of the residual in registers
+  static constexpr int AHEAD = TM < 2 || sizeof(T) == 4 ? 1 : 2;   // 32-row pieces of the residual in registers
   typedef row8 Residual[AHEAD][UNITS];
   static __device__ __forceinline__ void fetch(const MmP& p, int64_t m, int n, int lane, row8 (&res)[UNITS]) {
 #pragma unroll
@@ -334,7 +335,7 @@ template <typename T, int TM, int TN, bool PLAIN> struct WaveEpilogue {
   }
   // the first pieces of the residual: issued before the wave's last products
   static __device__ __forceinline__ void fetch_first(const MmP& p, int64_t m, int n, int lane, Residual& res) {
-    if (PLAIN || !p.residual) return;
+    if (!RES) return;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) fetch(p, m + 32 * i, n, lane, res[i]);
   }
@@ -369,10 +370,10 @@ template <typename T, int TM, int TN, bool PLAIN> struct WaveEpilogue {
           const int64_t at = row * p.N + c;
           if (PLAIN && p.slab) store_row<float, 8>(p.slab + (int64_t)t.split * p.M * p.N + at, left, v);
           else if (PLAIN) store_row<T, 8>(static_cast<T*>(p.y) + at, left, v);
-          else finish8<T, ACT>(p, at, left, v, bias, res[i % AHEAD][k]);
+          else finish8<T, ACT, RES>(p, at, left, v, bias, res[i % AHEAD][k]);
         }
       }
-      if (!PLAIN && p.residual && i + AHEAD < TM) fetch(p, m + 32 * (i + AHEAD), n, lane, res[i % AHEAD]);
+      if (RES && i + AHEAD < TM) fetch(p, m + 32 * (i + AHEAD), n, lane, res[i % AHEAD]);
       __builtin_amdgcn_wave_barrier();
     }
   }
@@ -391,14 +392,14 @@ template <typename T, int TM, int TN, bool PLAIN> struct WaveEpilogue {
 
 // WM x WN waves over the tile, WK waves over the reduction inside a step; NST stages in LDS, NST - 1 steps of loads in flight (DIRECT),
 // or loads through registers one step ahead with NST 1 or 2 stages.
-template <typename T, int BM, int BN, int BK, int WM, int WN, int WK, int LA, int LB, int NST, bool DIRECT>
-__global__ __launch_bounds__(WM * WN * WK * 64, 2) void mm_kernel(const MmP p) {
+template <typename T, int BM, int BN, int BK, int WM, int WN, int WK, int LA, int LB, int NST, bool DIRECT, bool RES>
+__global__ __launch_bounds__(WM * WN * WK * 64, DIRECT && NST == 3 ? 3 : 2) void mm_kernel(const MmP p) {
   constexpr int NTH = WM * WN * WK * 64, TM = BM / WM / 32, TN = BN / WN / 32, KS = BK / 16 / WK, NP = Frag<T>::NP;
   constexpr bool PLAIN = LB == LAY_R;                      // a gradient: no epilogue but the store
   typedef Operand<T, LA, BM, BK, NTH, DIRECT> OA;
   typedef Operand<T, LB, BN, BK, NTH, DIRECT> OB;
   typedef typename Frag<T>::F F;
-  typedef WaveEpilogue<T, TM, TN, PLAIN> WE;
+  typedef WaveEpilogue<T, TM, TN, PLAIN, RES> WE;
   static_assert(WK == 1 || (TM == 1 && TN == 1), "shared reductions: one tile a wave");
   constexpr int STAGE = OA::BYTES + OB::BYTES, EBYTES = WE::BYTES * WM * WN * WK;
   constexpr int LDS = NST * STAGE > EBYTES ? NST * STAGE : EBYTES;
@@ -650,32 +651,47 @@ int edge_of(int64_t m, int64_t n, int dtype) {
 // rows on 16-byte addresses, for the loads that write LDS themselves
 bool direct_ok(const void* base, int64_t ld, int es) { return ((uintptr_t)base & 15) == 0 && ld * es % 16 == 0; }
 
-template <typename T, int LA, int LB> void multiply(MmP& a, int edge, int splits, hipStream_t st) {
+template <typename T, int LA, int LB, bool RES> void multiply_as(MmP& a, int edge, int splits, hipStream_t st) {
   const bool direct = sizeof(T) == 2 && direct_ok(a.a, a.lda, 2) && direct_ok(a.b, a.ldb, 2);
   const bool wide = sizeof(T) == 4 && edge == 256;          // fp32: 128 x 256
-  // 256 x 256 forward: only over long reductions with little to load and store besides, as its two blocks of accumulators leave no
-  // registers for that (16384 x 2048 -> 2048, SiLU: 143 us, 128: 171; with residual and slope 203 and 187).
-  const bool lean = LB == LAY_R || (!a.residual && !a.slope && a.R >= 1024);
+  // 256 x 256 forward: not beside a residual, for which its accumulators leave no registers.  SiLU, bf16: 16384 x 2048 -> 2048 144 us,
+  // 128: 177; 32768 x 512 -> 2048 97 and 107, with its slope 134 and 143; 32768 x 256 -> 1024 39 and 43.
+  // 128 x 128 forward: three stages, so that three blocks share a CU and one's epilogue runs beside the others' products: 32768 x 512 ->
+  // 2048 with SiLU, slope and residual 160 us, with two blocks and three or four stages 173 to 175.  Gradients have a
+  // short epilogue and keep four stages (109 us, three: 113).
+  const bool lean = LB == LAY_R || (!RES && a.R >= 256);
   if (edge == 256 && !wide && !(direct && lean)) edge = 128;
   a.m_tiles = (int)cdiv(a.M, wide ? 128 : edge);
   a.n_tiles = (int)cdiv(a.N, edge);
   a.blocks = a.m_tiles * a.n_tiles * splits;
   const dim3 grid((unsigned)(cdiv(a.blocks, 8) * 8));
   if constexpr (sizeof(T) == 4) {
-    if (wide) hipLaunchKernelGGL((mm_kernel<T, 128, 256, 32, 2, 4, 1, LA, LB, 1, false>), grid, dim3(512), 0, st, a);
-    else if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
-    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 32, 2, 2, 1, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 1, false>), grid, dim3(256), 0, st, a);
+    if (wide) hipLaunchKernelGGL((mm_kernel<T, 128, 256, 32, 2, 4, 1, LA, LB, 1, false, RES>), grid, dim3(512), 0, st, a);
+    else if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 1, false, RES>), grid, dim3(256), 0, st, a);
+    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 32, 2, 2, 1, LA, LB, 1, false, RES>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 1, false, RES>), grid, dim3(256), 0, st, a);
   } else if (direct) {
-    if (edge == 256) hipLaunchKernelGGL((mm_kernel<T, 256, 256, 32, 2, 4, 1, LA, LB, 4, true>), grid, dim3(512), 0, st, a);
-    else if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, 4, true>), grid, dim3(256), 0, st, a);
-    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 64, 2, 2, 1, LA, LB, 4, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 8, true>), grid, dim3(256), 0, st, a);
+    if constexpr (!RES) {
+      if (edge == 256) {
+        hipLaunchKernelGGL((mm_kernel<T, 256, 256, 32, 2, 4, 1, LA, LB, 4, true, false>), grid, dim3(512), 0, st, a);
+        return;
+      }
+    }
+    if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 32, 2, 2, 1, LA, LB, LB == LAY_K ? 3 : 4, true, RES>), grid, dim3(256), 0, st, a);
+    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 64, 2, 2, 1, LA, LB, 4, true, RES>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 8, true, RES>), grid, dim3(256), 0, st, a);
   } else {
-    if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 64, 2, 2, 1, LA, LB, 2, false>), grid, dim3(256), 0, st, a);
-    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 64, 2, 2, 1, LA, LB, 2, false>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 2, false>), grid, dim3(256), 0, st, a);
+    if (edge == 128) hipLaunchKernelGGL((mm_kernel<T, 128, 128, 64, 2, 2, 1, LA, LB, 2, false, RES>), grid, dim3(256), 0, st, a);
+    else if (edge == 64) hipLaunchKernelGGL((mm_kernel<T, 64, 64, 64, 2, 2, 1, LA, LB, 2, false, RES>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mm_kernel<T, 32, 32, 64, 1, 1, 4, LA, LB, 2, false, RES>), grid, dim3(256), 0, st, a);
   }
+}
+
+template <typename T, int LA, int LB> void multiply(MmP& a, int edge, int splits, hipStream_t st) {
+  if constexpr (LB == LAY_K) {
+    if (a.residual) return multiply_as<T, LA, LB, true>(a, edge, splits, st);
+  }
+  multiply_as<T, LA, LB, false>(a, edge, splits, st);
 }
 
 struct Plan { int edge_x, edge_w, splits; int64_t r_split; int rows, parts; int64_t dz, part, slab, total; };
