@@ -23,8 +23,8 @@
 // three exact bf16 terms on their way to LDS and multiply in six products, like every intermediate beside them: 2^-23, and 2.7 times
 // the rate of the fp32 MFMA.
 //
-// Bound: by memory where there are many sequences (8192 of 32 tokens, 64 x 64, fp32, states in and out: 131 us for 0.54 GB, 4.1 TB/s;
-// their gradient, six products for each of its thirteen, 371 us for 0.87 GB), by the latency of one chunk after the other, about 4 us
+// Bound: by memory where there are many sequences (8192 of 32 tokens, 64 x 64, fp32, states in and out: 111 us for 0.54 GB, 4.8 TB/s;
+// their gradient, three scans in six-term products, 260 us for 0.87 GB), by the latency of one chunk after the other, about 4 us
 // in fp32 and 2 in 16 bits, where few sequences are long (8 of 16384 tokens, 128 x 128, bf16: 27 us for the segments' states, 11 to
 // join them, 57 for the outputs).
 //
@@ -318,11 +318,11 @@ struct Stage {
   }
 };
 
-// DP: both widths padded; STATE: only the segment's own contribution to the state; FULL: both widths are DP and
-// all rows lie on 16-byte addresses; PACK: sequences of one chunk, several to a block, the next one's loads under way during the
-// present one's products
-template <typename T, int DP, bool STATE, bool FULL, bool PACK>
-__global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
+// DP: both widths padded; STATE: only the segment's own contribution to the state; FULL: both widths are DP and all rows lie on 16-byte
+// addresses.  Full widths of 64 are held to 168 registers for a third wave on each SIMD (16384 sequences of 32 tokens, bf16: gradient
+// 272 us, 309 with two; 32768, fp32: forward 351 and 369, gradient 924 and 904).
+template <typename T, int DP, bool STATE, bool FULL>
+__global__ __launch_bounds__(DP / 16 * 64, DP == 64 && FULL && !STATE ? 3 : 2) void scan_kernel(const ScanP p) {
   typedef El<T> X;
   typedef typename X::Raw Raw;
   typedef typename X::In In;
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
   const Role& R = p.role[blockIdx.z];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
   const int split = blockIdx.y, t0 = split * p.seg, t1 = min(p.T, t0 + p.seg);
-  int bh = blockIdx.x;                                    // PACK: one of a run of (row, head), all of the same head
+  const int bh = blockIdx.x;
   const int h = bh % p.H, cw = wave * 16;                 // first value column of the wave
   const double l2 = log2_decay(p.log_decay, h);
   const int off = R.off, dq = FULL ? DP : R.dq, dv = FULL ? DP : R.dv;
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
   };
   int t = t0, n = min(C, t1 - t0);
   if (n > 0) fetch(bh, t, n);
-  f32x4 S[KT], Sn[PACK ? KT : 1];
+  f32x4 S[KT];
   load_state(bh, S);
   // lambda^n for every distance inside a chunk; scores weigh by lambda^(i-j): inside a diagonal tile directly, between tiles d + 1 apart
   // as lambda^(16 d + m + 1) * lambda^(15 - (4g + r)), both exponents non-negative
@@ -451,12 +451,7 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
       continue;
     }
     const int tn = t + n, nn = tn < careful ? 1 : min(C, t1 - tn);
-    const int next = PACK ? bh + (int)gridDim.x : p.BH;
     if (tn < t1) fetch(bh, tn, nn);
-    else if (PACK && next < p.BH) {
-      fetch(next, t0, t1 - t0);
-      load_state(next, reinterpret_cast<f32x4(&)[KT]>(Sn));
-    }
 
     // ---- the chunk's products (none for a wave whose columns are padding)
     if (cw < dv) {
@@ -544,14 +539,6 @@ __global__ __launch_bounds__(DP / 16 * 64, 2) void scan_kernel(const ScanP p) {
     __syncthreads();                                     // every wave has read the tiles
     t = tn;
     n = nn;
-    if (PACK && tn >= t1 && next < p.BH) {
-      store_state(bh, S);
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) S[kt] = Sn[PACK ? kt : 0];
-      bh = next;
-      t = careful = t0;
-      n = t1 - t0;
-    }
   }
   store_state(bh, S);
   if (STATE && tid == 0) p.flags[((int64_t)blockIdx.z * p.n_splits + split) * p.BH + bh] = any_reset;
@@ -650,7 +637,7 @@ __global__ __launch_bounds__(256) void step_kernel(const mrl_attention a, float*
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
-struct Plan { int dp, seg, n_splits, pack; };
+struct Plan { int dp, seg, n_splits; };
 
 int chunk_of(int dtype) { return dtype == MRL_F32 ? El<float>::C : El<__bf16>::C; }
 
@@ -696,11 +683,6 @@ Plan plan_of(const mrl_attention* p, int roles) {
   const int64_t per = std::max<int64_t>(1, cdiv(chunks, splits));
   r.seg = (int)(per * C);
   r.n_splits = (int)std::max<int64_t>(1, cdiv(chunks, per));
-  // Gradients of sequences of one chunk, more of them than the card holds blocks: that many blocks (a multiple of the heads) walk over
-  // them, with the next one's loads under way.  65536 sequences of 32 x 64: bf16 1218 us so and 1323 with a block each, fp32 1832 and
-  // 1918.  The forward pass (fp32 747 and 737) and narrow heads (32 x 32, 16 tokens, fp32: 601 and 488) keep a block each.
-  const int64_t resident = std::max<int64_t>(1, 2048 / waves / roles / p->heads) * p->heads;
-  r.pack = roles > 1 && r.dp == 64 && p->steps > 0 && chunks == 1 && p->batch * p->heads >= 2 * resident ? (int)resident : 0;
   return r;
 }
 
@@ -714,18 +696,12 @@ int64_t ws_bytes(const mrl_attention* p, const Plan& pl, int roles) {
 
 template <typename T, int DP, bool FULL> void launch_as(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
   const unsigned nth = DP / 16 * 64;
-  if constexpr (FULL && DP == 64) {
-    if (pl.pack > 0) {
-      hipLaunchKernelGGL((scan_kernel<T, DP, false, true, true>), dim3(pl.pack, 1, roles), dim3(nth), 0, st, a);
-      return;
-    }
-  }
   if (pl.n_splits > 1) {
-    hipLaunchKernelGGL((scan_kernel<T, DP, true, FULL, false>), dim3(a.BH, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
+    hipLaunchKernelGGL((scan_kernel<T, DP, true, FULL>), dim3(a.BH, pl.n_splits - 1, roles), dim3(nth), 0, st, a);
     const int64_t sz = (int64_t)a.role[0].dq * a.role[0].dv;
     hipLaunchKernelGGL(prefix_kernel, dim3((unsigned)cdiv(sz, 256), a.BH, roles), dim3(256), 0, st, a);
   }
-  hipLaunchKernelGGL((scan_kernel<T, DP, false, FULL, false>), dim3(a.BH, pl.n_splits, roles), dim3(nth), 0, st, a);
+  hipLaunchKernelGGL((scan_kernel<T, DP, false, FULL>), dim3(a.BH, pl.n_splits, roles), dim3(nth), 0, st, a);
 }
 template <typename T> void launch(const ScanP& a, const Plan& pl, int roles, hipStream_t st) {
   bool full = true;
