@@ -89,6 +89,14 @@ def test_large_tiles(dtype, shape):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('shape', [(13000, 264, 1000), (1100, 1048, 1032), (900, 1047, 1031), (700, 2056, 4104)])
+def test_large_tiles_without_a_residual(dtype, shape):
+    """The largest tiles forward, and those of 128 and 256 in the weight's gradient."""
+    check(*shape, DT[dtype], 'SiLU', 4, residual=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DT)
 @pytest.mark.parametrize('act', [None, 'SiLU', 'ELU', 'Tanh', 'GELU'])
 @pytest.mark.parametrize('bias,residual', [(True, True), (True, False), (False, True), (False, False)])
 def test_epilogues(dtype, act, bias, residual):
