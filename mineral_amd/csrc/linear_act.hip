@@ -529,8 +529,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64, DIRECT && NST == 3 ? 3 : 2) void
 }
 
 // dz = dy slope, rounded to T as an operand of the two products (with the results' own rounding that makes 1.4 times the error of one;
-// a second term would double both products: 180 us of 400 at 32768 x 512 -> 2048), and the sums of its columns, unrounded, over this block's rows -> part [blocks in y][N], or db where one block has all rows (a
-// launch less for small batches).  32 units of 8 columns x 8 rows a block.
+// a second term would double both products: 180 us of 400 at 32768 x 512 -> 2048), and the sums of its columns, unrounded, over this block's
+// rows -> part [blocks in y][N], or db where one block has all rows (a launch less for small batches).  32 units of 8 columns x 8 rows a block.
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* __restrict__ slope, const T* __restrict__ dy, T* __restrict__ dz, float* __restrict__ part,
                                                  T* __restrict__ db, int64_t M, int N, int rows) {
