@@ -4,11 +4,17 @@
 // environments takes less on the GPU than the interpreter needs to get there (17 us a call and 160 us for a call with its
 // gradient from Python on MI355X, measured with kernels of under 10 us).
 //
+// Every kernel is reached through the dispatcher, the forward pass below autograd and the backward pass from the autograd node: tracers,
+// dispatch modes, tensor subclasses and lazily negated tensors then see one operator instead of its allocations.  Operators whose names
+// begin with an underscore are the halves of a differentiable call.  Shape functions for tensors without data are in memory_ops.py.
+//
 // CPU tensors go through the same checks and are then refused: there is no CPU kernel.
 #include "../../include/mineral_memory.h"
 #include "../../include/mineral_ppo.h"
 
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -85,11 +91,32 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// The operator `name` as a typed handle, and a call of it below autograd.
+template <typename Signature> c10::TypedOperatorHandle<Signature> op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+using BelowAutograd = at::AutoDispatchBelowAutograd;
+
 void once(const char* what) {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, ": differentiable once; its gradient under create_graph=True has none of its own");
 }
 
 [[noreturn]] void no_cpu(const char* what) { TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": tensors have to be on the GPU, there is no CPU kernel"); }
+
+// Of tensors in the order of the bits of `needs`: those whose bit is set, and back to where they belong.
+std::vector<Tensor> asked(int64_t needs, std::initializer_list<Tensor> all) {
+  std::vector<Tensor> r;
+  int i = 0;
+  for (const Tensor& t : all)
+    if (needs >> i++ & 1) r.push_back(t);
+  return r;
+}
+void place(int64_t needs, const std::vector<Tensor>& got, std::initializer_list<Tensor*> to) {
+  size_t n = 0;
+  int i = 0;
+  for (Tensor* t : to)
+    if (needs >> i++ & 1) *t = got[n++];
+}
 
 // ---- linear attention ------------------------------------------------------------------------------------------------------------
 struct Attention {
@@ -142,54 +169,70 @@ struct Attention {
   Tensor new_state() const { return new_floats(q, {a.batch, a.heads, a.dim_k, a.dim_v}); }
 };
 
-std::tuple<Tensor, Tensor> attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& r, const Tensor& s, double scale) {
+std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale) {
   const char* what = "linear_attention";
-  const Attention d(what, q, k, v, l, r, s, scale, false);
+  const Attention d(what, q, k, v, l, of(r), of(s), scale, false);
   c10::DeviceGuard guard(q.device());
   Tensor out = new_like(v, v.sizes()), final = d.new_state();
   const Workspace ws(what, mrl_linear_attention_workspace_bytes(&d.a, 0), q);
   check(mrl_linear_attention(&d.a, mp(out), static_cast<float*>(mp(final)), ws.p(), ws.n, stream_of(q)), what);
   return {out, final};
 }
+using AttentionSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptT&, const OptT&, double);
+
+// The gradients that `needs` names (1 q, 2 k, 4 v, 8 initial state), in this order.
+std::vector<Tensor> attention_backward(const OptT& dout_, const OptT& dfinal_, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s,
+                                       double scale, int64_t needs) {
+  const char* what = "linear_attention_backward";
+  const Attention d(what, q, k, v, l, of(r), of(s), scale, false);
+  c10::DeviceGuard guard(q.device());
+  const Tensor dout = dout_.has_value() ? rows_of(*dout_) : at::zeros_like(v, at::MemoryFormat::Contiguous), dfinal = contiguous(of(dfinal_));
+  const int64_t st[3] = {dout.stride(0), dout.stride(1), dout.stride(2)};
+  Tensor dq, dk, ds;
+  if (needs & 1) dq = new_like(q, q.sizes());
+  if (needs & 2) dk = new_like(k, k.sizes());
+  Tensor dv = needs & 12 ? new_like(v, v.sizes()) : Tensor();             // the state's gradient comes with it
+  if (needs & 8) ds = d.new_state();
+  const Workspace ws(what, mrl_linear_attention_workspace_bytes(&d.a, 1), q);
+  check(mrl_linear_attention_backward(&d.a, cp(dout), st, static_cast<const float*>(cp(dfinal)), mp(dq), mp(dk), mp(dv), static_cast<float*>(mp(ds)), ws.p(), ws.n, stream_of(q)),
+        what);
+  return asked(needs, {dq, dk, dv, ds});
+}
+using AttentionBackwardSig = std::vector<Tensor>(const OptT&, const OptT&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptT&, const OptT&, double, int64_t);
 
 struct LinearAttention : Function<LinearAttention> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale,
                                int64_t needs) {
+    static const auto fwd = op<AttentionSig>("mineral::linear_attention");
+    const BelowAutograd below;
     ctx->set_materialize_grads(false);
-    auto [out, final] = attention_forward(q, k, v, l, of(r), of(s), scale);
+    auto [out, final] = fwd.call(q, k, v, l, r, s, scale);
     ctx->save_for_backward({q, k, v, l, of(r), of(s)});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["needs"] = needs;
     return {out, final};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const char* what = "linear_attention_backward";
+    static const auto bwd = op<AttentionBackwardSig>("mineral::_linear_attention_backward");
     once("linear_attention");
     variable_list res(8);
     if (!g[0].defined() && !g[1].defined()) return res;
+    const BelowAutograd below;
     const auto t = ctx->get_saved_variables();
     const int64_t needs = ctx->saved_data["needs"].toInt();
-    const Attention d(what, t[0], t[1], t[2], t[3], t[4], t[5], ctx->saved_data["scale"].toDouble(), false);
-    c10::DeviceGuard guard(t[0].device());
-    const Tensor dout = g[0].defined() ? rows_of(g[0]) : at::zeros_like(t[2], at::MemoryFormat::Contiguous), dfinal = contiguous(g[1]);
-    const int64_t st[3] = {dout.stride(0), dout.stride(1), dout.stride(2)};
-    if (needs & 1) res[0] = new_like(t[0], t[0].sizes());
-    if (needs & 2) res[1] = new_like(t[1], t[1].sizes());
-    Tensor dv = needs & 12 ? new_like(t[2], t[2].sizes()) : Tensor();     // the state's gradient comes with it
-    if (needs & 4) res[2] = dv;
-    if (needs & 8) res[5] = d.new_state();
-    const Workspace ws(what, mrl_linear_attention_workspace_bytes(&d.a, 1), t[0]);
-    check(mrl_linear_attention_backward(&d.a, cp(dout), st, static_cast<const float*>(cp(dfinal)), mp(res[0]), mp(res[1]), mp(dv), static_cast<float*>(mp(res[5])), ws.p(),
-                                        ws.n, stream_of(t[0])), what);
+    const auto got = bwd.call(opt(g[0]), opt(g[1]), t[0], t[1], t[2], t[3], opt(t[4]), opt(t[5]), ctx->saved_data["scale"].toDouble(), needs);
+    place(needs, got, {&res[0], &res[1], &res[2], &res[5]});
     return res;
   }
 };
 
-std::tuple<Tensor, Tensor> linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale) {
-  return attention_forward(q, k, v, l, of(r), of(s), scale);
-}
-std::tuple<Tensor, Tensor> linear_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s, double scale) {
-  if (!wants_grad({&q, &k, &v, &l, &of(s)})) return attention_forward(q, k, v, l, of(r), of(s), scale);
+std::tuple<Tensor, Tensor> linear_attention_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s,
+                                                     double scale) {
+  if (!wants_grad({&q, &k, &v, &l, &of(s)})) {
+    static const auto fwd = op<AttentionSig>("mineral::linear_attention");
+    const BelowAutograd below;
+    return fwd.redispatch(ks & c10::after_autograd_keyset, q, k, v, l, r, s, scale);
+  }
   TORCH_CHECK_NOT_IMPLEMENTED(!l.requires_grad(), "linear_attention: the decays are constants of the heads; log_decay has no gradient");
   const int64_t needs = q.requires_grad() | k.requires_grad() << 1 | v.requires_grad() << 2 | (of(s).defined() && s->requires_grad()) << 3;
   const auto o = LinearAttention::apply(q, k, v, l, r, s, scale, needs);
@@ -202,13 +245,39 @@ std::tuple<Tensor, Tensor> linear_attention_cpu(const Tensor& q, const Tensor& k
 
 Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
   const char* what = "linear_attention_step";
-  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({&q, &k, &v, &l, &state}), what, ": no gradient (linear_attention over the rollout has one); call it under torch.no_grad()");
   const Attention d(what, q, k, v, l, of(r), state, scale, true);
   if (q.is_cpu()) no_cpu(what);
   c10::DeviceGuard guard(q.device());
-  state.unsafeGetTensorImpl()->bump_version();                            // written below torch's own bookkeeping
   Tensor out = new_like(v, v.sizes());
   check(mrl_linear_attention_step(&d.a, static_cast<float*>(mp(state)), mp(out), stream_of(q)), what);
+  return out;
+}
+using StepSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptT&, double);
+
+Tensor linear_attention_step_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
+  static const auto fwd = op<StepSig>("mineral::linear_attention_step");
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({&q, &k, &v, &l, &state}),
+                              "linear_attention_step: no gradient (linear_attention over the rollout has one); call it under torch.no_grad()");
+  const BelowAutograd below;
+  return fwd.redispatch(ks & c10::after_autograd_keyset, q, k, v, l, state, r, scale);
+}
+// Reached in inference mode too, where autograd is not: what a step overwrites is marked as written.
+Tensor linear_attention_step_inplace(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
+  static const auto fwd = op<StepSig>("mineral::linear_attention_step");
+  Tensor out;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    out = fwd.redispatch(ks & c10::after_ADInplaceOrView_keyset, q, k, v, l, state, r, scale);
+  }
+  state.unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+// torch's own fallback for lazily negated tensors serves operators that return what they overwrite; this one returns something else.
+Tensor linear_attention_step_negated(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
+  static const auto fwd = op<StepSig>("mineral::linear_attention_step");
+  const Tensor s = state.resolve_neg();
+  Tensor out = fwd.call(q.resolve_neg(), k.resolve_neg(), v.resolve_neg(), l.resolve_neg(), s, r, scale);
+  if (state.is_neg()) state.copy_(s);
   return out;
 }
 
@@ -257,9 +326,46 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x_, int64_t groups, const 
   return {y, stats};
 }
 
+using Name = std::optional<std::string_view>;
+
+Tensor group_norm_act(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
+  return std::get<0>(norm_forward(x, groups, of(w), of(b), eps, act_of("group_norm_act", act), false));
+}
+using NormSig = Tensor(const Tensor&, int64_t, const OptT&, const OptT&, double, Name);
+
+std::tuple<Tensor, Tensor> group_norm_act_stats(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, int64_t act) {
+  return norm_forward(x, groups, of(w), of(b), eps, (int)act, true);
+}
+using NormStatsSig = std::tuple<Tensor, Tensor>(const Tensor&, int64_t, const OptT&, const OptT&, double, int64_t);
+
+// The gradients that `needs` names (1 x, 2 weight, 4 bias), in this order.
+std::vector<Tensor> group_norm_act_backward(const Tensor& dy_, const Tensor& x_, const Tensor& stats, const OptT& w_, const OptT& b_, int64_t groups, double eps, int64_t act,
+                                            int64_t needs) {
+  const char* what = "group_norm_act_backward";
+  const mrl_group_norm p = norm_of(what, x_, groups, of(w_), of(b_), eps, (int)act);
+  c10::DeviceGuard guard(x_.device());
+  const Tensor x = aligned(x_), dy = aligned(dy_), w = contiguous(of(w_)), b = contiguous(of(b_));
+  Tensor dx = new_like(x, x.sizes()), dw, db;
+  if (needs & 6) {
+    const auto o = x.options().dtype(p.param_dtype == MRL_F32 ? at::kFloat : x.scalar_type()).requires_grad(false);
+    const bool empty = x.numel() == 0;
+    dw = empty ? at::zeros({p.channels}, o) : at::empty({p.channels}, o);
+    db = empty ? at::zeros({p.channels}, o) : at::empty({p.channels}, o);
+  }
+  if (x.numel() > 0) {
+    const Workspace ws(what, mrl_group_norm_act_workspace_bytes(&p, 1), x);
+    const float* mean = static_cast<const float*>(cp(stats));
+    check(mrl_group_norm_act_backward(&p, cp(x), cp(dy), cp(w), cp(b), mean, mean + p.batch * p.groups, mp(dx), mp(dw), mp(db), ws.p(), ws.n, stream_of(x)), what);
+  }
+  return asked(needs, {dx, dw, db});
+}
+using NormBackwardSig = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptT&, const OptT&, int64_t, double, int64_t, int64_t);
+
 struct GroupNormAct : Function<GroupNormAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptT& w, const OptT& b, int64_t groups, double eps, int64_t act, int64_t needs) {
-    auto [y, stats] = norm_forward(x, groups, of(w), of(b), eps, (int)act, true);
+    static const auto fwd = op<NormStatsSig>("mineral::_group_norm_act_stats");
+    const BelowAutograd below;
+    auto [y, stats] = fwd.call(x, groups, w, b, eps, act);
     ctx->save_for_backward({x, stats, of(w), of(b)});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["eps"] = eps;
@@ -268,45 +374,33 @@ struct GroupNormAct : Function<GroupNormAct> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const char* what = "group_norm_act_backward";
+    static const auto bwd = op<NormBackwardSig>("mineral::_group_norm_act_backward");
     once("group_norm_act");
+    const BelowAutograd below;
     const auto t = ctx->get_saved_variables();
     const int64_t needs = ctx->saved_data["needs"].toInt();
-    const mrl_group_norm p = norm_of(what, t[0], ctx->saved_data["groups"].toInt(), t[2], t[3], ctx->saved_data["eps"].toDouble(), (int)ctx->saved_data["act"].toInt());
-    c10::DeviceGuard guard(t[0].device());
-    const Tensor x = aligned(t[0]), dy = aligned(g[0]), w = contiguous(t[2]), b = contiguous(t[3]);
-    Tensor dx = new_like(x, x.sizes()), dw, db;
-    if (needs & 6) {
-      const auto o = x.options().dtype(p.param_dtype == MRL_F32 ? at::kFloat : x.scalar_type()).requires_grad(false);
-      const bool empty = x.numel() == 0;
-      dw = empty ? at::zeros({p.channels}, o) : at::empty({p.channels}, o);
-      db = empty ? at::zeros({p.channels}, o) : at::empty({p.channels}, o);
-    }
-    if (x.numel() > 0) {
-      const Workspace ws(what, mrl_group_norm_act_workspace_bytes(&p, 1), x);
-      const float* mean = static_cast<const float*>(cp(t[1]));
-      check(mrl_group_norm_act_backward(&p, cp(x), cp(dy), cp(w), cp(b), mean, mean + p.batch * p.groups, mp(dx), mp(dw), mp(db), ws.p(), ws.n, stream_of(x)), what);
-    }
     variable_list res(7);
-    res[0] = dx;
-    if (needs & 2) res[1] = dw;
-    if (needs & 4) res[2] = db;
+    const auto got = bwd.call(g[0], t[0], t[1], opt(t[2]), opt(t[3]), ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["act"].toInt(), needs);
+    place(needs, got, {&res[0], &res[1], &res[2]});
     return res;
   }
 };
 
-using Name = std::optional<std::string_view>;
-
-Tensor group_norm_act(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
-  return std::get<0>(norm_forward(x, groups, of(w), of(b), eps, act_of("group_norm_act", act), false));
-}
-Tensor group_norm_act_autograd(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
-  if (!wants_grad({&x, &of(w), &of(b)})) return group_norm_act(x, groups, w, b, eps, act);
+Tensor group_norm_act_autograd(c10::DispatchKeySet ks, const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
+  if (!wants_grad({&x, &of(w), &of(b)})) {
+    static const auto fwd = op<NormSig>("mineral::group_norm_act");
+    const BelowAutograd below;
+    return fwd.redispatch(ks & c10::after_autograd_keyset, x, groups, w, b, eps, act);
+  }
   const int64_t needs = x.requires_grad() | (of(w).defined() && w->requires_grad()) << 1 | (of(b).defined() && b->requires_grad()) << 2;
   return GroupNormAct::apply(x, w, b, groups, eps, (int64_t)act_of("group_norm_act", act), needs);
 }
 Tensor group_norm_act_cpu(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
   norm_of("group_norm_act", x, groups, of(w), of(b), eps, act_of("group_norm_act", act));
+  no_cpu("group_norm_act");
+}
+std::tuple<Tensor, Tensor> group_norm_act_stats_cpu(const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, int64_t act) {
+  norm_of("group_norm_act", x, groups, of(w), of(b), eps, (int)act);
   no_cpu("group_norm_act");
 }
 
@@ -353,48 +447,84 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w_, con
   return {y, slope};
 }
 
+Tensor linear_act(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
+  return std::get<0>(linear_forward(x, w, of(b), of(r), act_of("linear_act", act), false));
+}
+using LinearSig = Tensor(const Tensor&, const Tensor&, const OptT&, const OptT&, Name);
+
+std::tuple<Tensor, Tensor> linear_act_slope(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, int64_t act) {
+  TORCH_CHECK_VALUE(act != MRL_ACT_NONE, "linear_act: no activation, no slope");
+  return linear_forward(x, w, of(b), of(r), (int)act, true);
+}
+using LinearSlopeSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptT&, const OptT&, int64_t);
+
+// The gradients that `needs` names (1 x, 2 weight, 4 bias), in this order.
+std::vector<Tensor> linear_act_backward(const Tensor& dy_, const Tensor& x, const Tensor& w_, const OptT& slope, int64_t act, int64_t needs) {
+  const char* what = "linear_act_backward";
+  const Linear d(what, x, w_, none, none, (int)act);
+  c10::DeviceGuard guard(x.device());
+  Tensor dx, dw, db;
+  if (needs & 1) dx = new_like(x, x.sizes());
+  if (needs & 2) dw = new_like(w_, w_.sizes());
+  if (needs & 4) db = new_like(x, {d.p.outputs});
+  if (d.p.outputs == 0) {
+    if (dx.defined()) dx.zero_();
+  } else {
+    const Tensor w = w_.contiguous(), dy = dy_.contiguous();
+    const Workspace ws(what, mrl_linear_act_backward_workspace_bytes(&d.p), dy);
+    check(mrl_linear_act_backward(&d.p, cp(d.x), cp(w), cp(of(slope)), cp(dy), mp(dx), mp(dw), mp(db), ws.p(), ws.n, stream_of(dy)), what);
+  }
+  return asked(needs, {dx, dw, db});
+}
+using LinearBackwardSig = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptT&, int64_t, int64_t);
+
 struct LinearAct : Function<LinearAct> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, int64_t act, int64_t needs) {
-    auto [y, slope] = linear_forward(x, w, of(b), of(r), (int)act, needs & 7);
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name name, int64_t needs) {
+    const int act = act_of("linear_act", name);
+    const BelowAutograd below;
+    Tensor y, slope;
+    if (act != MRL_ACT_NONE && needs & 7) {
+      static const auto fwd = op<LinearSlopeSig>("mineral::_linear_act_slope");
+      std::tie(y, slope) = fwd.call(x, w, b, r, act);
+    } else {
+      static const auto fwd = op<LinearSig>("mineral::linear_act");
+      y = fwd.call(x, w, b, r, name);
+    }
     ctx->save_for_backward({x, w, slope});
-    ctx->saved_data["act"] = act;
+    ctx->saved_data["act"] = (int64_t)act;
     ctx->saved_data["needs"] = needs;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const char* what = "linear_act_backward";
+    static const auto bwd = op<LinearBackwardSig>("mineral::_linear_act_backward");
     once("linear_act");
     variable_list res(6);
     const int64_t needs = ctx->saved_data["needs"].toInt();
     if (needs & 8) res[3] = g[0];
     if (!(needs & 7)) return res;
+    const BelowAutograd below;
     const auto t = ctx->get_saved_variables();
-    const Linear d(what, t[0], t[1], none, none, (int)ctx->saved_data["act"].toInt());
-    c10::DeviceGuard guard(t[0].device());
-    if (needs & 1) res[0] = new_like(t[0], t[0].sizes());
-    if (needs & 2) res[1] = new_like(t[1], t[1].sizes());
-    if (needs & 4) res[2] = new_like(t[0], {d.p.outputs});
-    if (d.p.outputs == 0) {
-      if (res[0].defined()) res[0].zero_();
-      return res;
-    }
-    const Tensor w = t[1].contiguous(), dy = g[0].contiguous();
-    const Workspace ws(what, mrl_linear_act_backward_workspace_bytes(&d.p), dy);
-    check(mrl_linear_act_backward(&d.p, cp(d.x), cp(w), cp(t[2]), cp(dy), mp(res[0]), mp(res[1]), mp(res[2]), ws.p(), ws.n, stream_of(dy)), what);
+    const auto got = bwd.call(g[0], t[0], t[1], opt(t[2]), ctx->saved_data["act"].toInt(), needs & 7);
+    place(needs & 7, got, {&res[0], &res[1], &res[2]});
     return res;
   }
 };
 
-Tensor linear_act(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
-  return std::get<0>(linear_forward(x, w, of(b), of(r), act_of("linear_act", act), false));
-}
-Tensor linear_act_autograd(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
-  if (!wants_grad({&x, &w, &of(b), &of(r)})) return linear_act(x, w, b, r, act);
+Tensor linear_act_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
+  if (!wants_grad({&x, &w, &of(b), &of(r)})) {
+    static const auto fwd = op<LinearSig>("mineral::linear_act");
+    const BelowAutograd below;
+    return fwd.redispatch(ks & c10::after_autograd_keyset, x, w, b, r, act);
+  }
   const int64_t needs = x.requires_grad() | w.requires_grad() << 1 | (of(b).defined() && b->requires_grad()) << 2 | (of(r).defined() && r->requires_grad()) << 3;
-  return LinearAct::apply(x, w, b, r, (int64_t)act_of("linear_act", act), needs);
+  return LinearAct::apply(x, w, b, r, act, needs);
 }
 Tensor linear_act_cpu(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
   const Linear d("linear_act", x, w, of(b), of(r), act_of("linear_act", act));
+  no_cpu("linear_act");
+}
+std::tuple<Tensor, Tensor> linear_act_slope_cpu(const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, int64_t act) {
+  const Linear d("linear_act", x, w, of(b), of(r), (int)act);
   no_cpu("linear_act");
 }
 
@@ -405,22 +535,37 @@ TORCH_LIBRARY_FRAGMENT(mineral, m) {
   m.def("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, Tensor? resets=None, float scale=1.0) -> Tensor");
   m.def("group_norm_act(Tensor x, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, str? act_type=None) -> Tensor");
   m.def("linear_act(Tensor x, Tensor weight, Tensor? bias=None, Tensor? residual=None, str? act_type=None) -> Tensor");
+  // the halves of a differentiable call
+  m.def("_linear_attention_backward(Tensor? d_out, Tensor? d_final, Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? resets, Tensor? initial_state, float scale, int needs) -> Tensor[]");
+  m.def("_group_norm_act_stats(Tensor x, int num_groups, Tensor? weight, Tensor? bias, float eps, int act) -> (Tensor, Tensor)");
+  m.def("_group_norm_act_backward(Tensor dy, Tensor x, Tensor stats, Tensor? weight, Tensor? bias, int num_groups, float eps, int act, int needs) -> Tensor[]");
+  m.def("_linear_act_slope(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act) -> (Tensor, Tensor)");
+  m.def("_linear_act_backward(Tensor dy, Tensor x, Tensor weight, Tensor? slope, int act, int needs) -> Tensor[]");
 }
 TORCH_LIBRARY_IMPL(mineral, CUDA, m) {
   m.impl("linear_attention", linear_attention);
   m.impl("linear_attention_step", linear_attention_step);
   m.impl("group_norm_act", group_norm_act);
   m.impl("linear_act", linear_act);
+  m.impl("_linear_attention_backward", attention_backward);
+  m.impl("_group_norm_act_stats", group_norm_act_stats);
+  m.impl("_group_norm_act_backward", group_norm_act_backward);
+  m.impl("_linear_act_slope", linear_act_slope);
+  m.impl("_linear_act_backward", linear_act_backward);
 }
-TORCH_LIBRARY_IMPL(mineral, AutogradCUDA, m) {
+TORCH_LIBRARY_IMPL(mineral, Autograd, m) {
   m.impl("linear_attention", linear_attention_autograd);
-  m.impl("linear_attention_step", linear_attention_step);
+  m.impl("linear_attention_step", linear_attention_step_autograd);
   m.impl("group_norm_act", group_norm_act_autograd);
   m.impl("linear_act", linear_act_autograd);
 }
+TORCH_LIBRARY_IMPL(mineral, ADInplaceOrView, m) { m.impl("linear_attention_step", linear_attention_step_inplace); }
+TORCH_LIBRARY_IMPL(mineral, Negative, m) { m.impl("linear_attention_step", linear_attention_step_negated); }
 TORCH_LIBRARY_IMPL(mineral, CPU, m) {
   m.impl("linear_attention", linear_attention_cpu);
   m.impl("linear_attention_step", linear_attention_step);
   m.impl("group_norm_act", group_norm_act_cpu);
   m.impl("linear_act", linear_act_cpu);
+  m.impl("_group_norm_act_stats", group_norm_act_stats_cpu);
+  m.impl("_linear_act_slope", linear_act_slope_cpu);
 }
