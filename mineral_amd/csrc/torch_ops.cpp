@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -89,6 +90,13 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Forward-mode derivatives are refused instead of dropped.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, ": no forward-mode derivative");
 }
 
 // The operator `name` as a typed handle, and a call of it below autograd.
@@ -215,6 +223,7 @@ struct LinearAttention : Function<LinearAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     static const auto bwd = op<AttentionBackwardSig>("mineral::_linear_attention_backward");
     once("linear_attention");
+    no_tangent("linear_attention", {&g[0], &g[1]});
     variable_list res(8);
     if (!g[0].defined() && !g[1].defined()) return res;
     const BelowAutograd below;
@@ -228,6 +237,7 @@ struct LinearAttention : Function<LinearAttention> {
 
 std::tuple<Tensor, Tensor> linear_attention_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const OptT& r, const OptT& s,
                                                      double scale) {
+  no_tangent("linear_attention", {&q, &k, &v, &l, &of(s)});
   if (!wants_grad({&q, &k, &v, &l, &of(s)})) {
     static const auto fwd = op<AttentionSig>("mineral::linear_attention");
     const BelowAutograd below;
@@ -256,6 +266,7 @@ using StepSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor
 
 Tensor linear_attention_step_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
   static const auto fwd = op<StepSig>("mineral::linear_attention_step");
+  no_tangent("linear_attention_step", {&q, &k, &v, &l, &state});
   TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({&q, &k, &v, &l, &state}),
                               "linear_attention_step: no gradient (linear_attention over the rollout has one); call it under torch.no_grad()");
   const BelowAutograd below;
@@ -376,6 +387,7 @@ struct GroupNormAct : Function<GroupNormAct> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     static const auto bwd = op<NormBackwardSig>("mineral::_group_norm_act_backward");
     once("group_norm_act");
+    no_tangent("group_norm_act", {&g[0]});
     const BelowAutograd below;
     const auto t = ctx->get_saved_variables();
     const int64_t needs = ctx->saved_data["needs"].toInt();
@@ -387,6 +399,7 @@ struct GroupNormAct : Function<GroupNormAct> {
 };
 
 Tensor group_norm_act_autograd(c10::DispatchKeySet ks, const Tensor& x, int64_t groups, const OptT& w, const OptT& b, double eps, Name act) {
+  no_tangent("group_norm_act", {&x, &of(w), &of(b)});
   if (!wants_grad({&x, &of(w), &of(b)})) {
     static const auto fwd = op<NormSig>("mineral::group_norm_act");
     const BelowAutograd below;
@@ -498,6 +511,7 @@ struct LinearAct : Function<LinearAct> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     static const auto bwd = op<LinearBackwardSig>("mineral::_linear_act_backward");
     once("linear_act");
+    no_tangent("linear_act", {&g[0]});
     variable_list res(6);
     const int64_t needs = ctx->saved_data["needs"].toInt();
     if (needs & 8) res[3] = g[0];
@@ -511,6 +525,7 @@ struct LinearAct : Function<LinearAct> {
 };
 
 Tensor linear_act_autograd(c10::DispatchKeySet ks, const Tensor& x, const Tensor& w, const OptT& b, const OptT& r, Name act) {
+  no_tangent("linear_act", {&x, &w, &of(b), &of(r)});
   if (!wants_grad({&x, &w, &of(b), &of(r)})) {
     static const auto fwd = op<LinearSig>("mineral::linear_act");
     const BelowAutograd below;

@@ -139,3 +139,52 @@ def test_a_gradient_that_arrives_lazily_negated(name):
     want = torch.autograd.grad(out, leaves, g, retain_graph=True)
     got = torch.autograd.grad(out, leaves, [negated(t) for t in g])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def dual(name, device, i):
+    """The call with a tangent on input i, inside a dual level."""
+    import torch.autograd.forward_ad as fwd
+    call, _, args = inputs(device)[name]
+    with fwd.dual_level():
+        return call(*[fwd.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)])
+
+
+@pytest.mark.parametrize('name', NAMES)
+def test_a_forward_mode_derivative_is_refused(name):
+    """Before anything else is asked, the device among it."""
+    for i in range(len(inputs('cpu')[name][2])):
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            dual(name, 'cpu', i)
+        with pytest.raises(NotImplementedError, match='forward-mode'), torch.no_grad():
+            dual(name, 'cpu', i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', NAMES)
+def test_a_forward_mode_derivative_is_refused_on_the_device(name):
+    import torch.autograd.forward_ad as fwd
+    call, where, args = inputs()[name]
+    for i in range(len(args)):
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            dual(name, DEV, i)
+    # a tangent that arrives with the gradient
+    if where:
+        leaves = [t.clone().requires_grad_(True) if i in where else t for i, t in enumerate(args)]
+        out = flat(call(*leaves))
+        with fwd.dual_level():
+            g = [fwd.make_dual(torch.ones_like(t), torch.ones_like(t)) for t in out]
+            with pytest.raises(NotImplementedError, match='forward-mode'):
+                torch.autograd.grad(out, [leaves[i] for i in where], g)
+    # a dual level without tangents, and tangents that are switched off, change nothing
+    want = flat(call(*[t.clone() for t in args]))
+    with fwd.dual_level():
+        assert all(torch.equal(a, b) for a, b in zip(flat(call(*[t.clone() for t in args])), want))
+        with fwd._set_fwd_grad_enabled(False):
+            assert all(torch.equal(a, b) for a, b in zip(flat(call(*[t.clone() for t in args])), want))
+
+
+@pytest.mark.parametrize('name', HALVES)
+def test_a_functional_jvp_is_refused(name):
+    call, where, args = inputs('cpu')[name]
+    with pytest.raises(NotImplementedError, match='forward-mode'):
+        torch.func.jvp(lambda t: call(t, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
