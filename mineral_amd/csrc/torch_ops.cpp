@@ -546,6 +546,7 @@ std::tuple<Tensor, Tensor> linear_act_slope_cpu(const Tensor& x, const Tensor& w
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mineral, m) {
+  m.set_python_module("mineral_amd.memory_ops");            // where the shape functions are
   m.def("linear_attention(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? resets=None, Tensor? initial_state=None, float scale=1.0) -> (Tensor, Tensor)");
   m.def("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, Tensor? resets=None, float scale=1.0) -> Tensor");
   m.def("group_norm_act(Tensor x, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, str? act_type=None) -> Tensor");

@@ -188,3 +188,98 @@ def test_a_functional_jvp_is_refused(name):
     call, where, args = inputs('cpu')[name]
     with pytest.raises(NotImplementedError, match='forward-mode'):
         torch.func.jvp(lambda t: call(t, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
+
+
+def shapes(outs):
+    return [(tuple(t.shape), t.dtype, t.is_contiguous()) for t in outs]
+
+
+EXPECTED = {'linear_attention': [(2, 5, 3, 12), (2, 3, 8, 12)], 'linear_attention_step': [(2, 3, 12)], 'group_norm_act': [(6, 32)], 'linear_act': [(6, 24)]}
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('name', NAMES)
+def test_shapes_of_tensors_without_data(name, dtype):
+    call, where, args = inputs('meta', dtype)[name]
+    out = flat(call(*args))
+    assert [tuple(t.shape) for t in out] == EXPECTED[name] and all(t.is_meta and t.is_contiguous() for t in out)
+    assert out[0].dtype == dtype and (len(out) == 1 or out[1].dtype == torch.float32)
+    if where:
+        run, args = with_gradient(name, 'meta', dtype)
+        got = run(*args)
+        assert shapes(got[len(out):]) == [(tuple(args[i].shape), args[i].dtype, True) for i in where]
+
+
+@pytest.mark.parametrize('name', NAMES)
+def test_a_trace_without_data_records_the_operator(name):
+    """Tensors of a device that need not be there, and, with the gradient, of none."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, where, args = inputs('meta')[name]
+    if name != 'linear_attention':          # whose resets are a constant of the call
+        with FakeTensorMode():
+            on_device = [torch.empty(t.shape, dtype=t.dtype, device=DEV) for t in args]
+            assert f'torch.ops.mineral.{name}' in make_fx(lambda *a: tuple(2 * t for t in flat(call(*a))))(*on_device).code
+    if where:
+        run, args = with_gradient(name, 'meta')
+        code = make_fx(run)(*args).code
+        assert all(f'torch.ops.mineral.{h}.' in code for h in HALVES[name]) and 'aten.empty.' not in code
+
+
+def test_symbolic_sizes():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    M = ops()
+    for name, fn, args in (('linear_act', lambda x, w: M.linear_act(x, w, None, None, 'SiLU'), [torch.empty(6, 16, device='meta'), torch.empty(24, 16, device='meta')]),
+                           ('group_norm_act', lambda x: M.group_norm_act(x, 4, None, None, 1e-5, None), [torch.empty(6, 9, 32, device='meta')]),
+                           ('linear_attention', lambda q, k, v, l: M.linear_attention(q, k, v, l)[1], [torch.empty(2, 5, 3, 8, device='meta')] * 2 + [torch.empty(2, 5, 3, 12, device='meta'), torch.empty(3, device='meta')])):
+        graph = make_fx(fn, tracing_mode='symbolic')(*args)
+        assert f'torch.ops.mineral.{name}' in graph.code
+        more = [t.new_empty((7, *t.shape[1:])) if t.dim() > 2 or name == 'linear_act' and i == 0 else t for i, t in enumerate(args)]
+        assert graph(*more).shape == fn(*more).shape and graph(*more).shape[0] == 7
+
+
+def test_shapes_that_do_not_fit_are_refused_without_data():
+    M = ops()
+    e = lambda *s, **k: torch.empty(*s, device='meta', **k)  # noqa: E731
+    for bad in (lambda: M.linear_act(e(4, 8), e(6, 7)), lambda: M.linear_act(e(4, 8), e(6, 8), e(5)), lambda: M.linear_act(e(4, 8), e(6, 8), None, e(1, 6)),
+                lambda: M.linear_act(e(4, 8), e(6, 8, dtype=torch.half)), lambda: M.group_norm_act(e(4, 9), 2), lambda: M.group_norm_act(e(4, 8), 2, e(4)),
+                lambda: M.linear_attention(e(2, 4, 2, 8), e(2, 4, 2, 8), e(2, 3, 2, 8), e(2)), lambda: M.linear_attention(e(2, 4, 2, 8), e(2, 4, 2, 8), e(2, 4, 2, 8), e(3)),
+                lambda: M.linear_attention_step(e(2, 2, 8), e(2, 2, 8), e(2, 2, 8), e(2), e(2, 2, 8, 4)), lambda: M.linear_act(e(4, 8, dtype=torch.double), e(6, 8, dtype=torch.double))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', NAMES)
+def test_shape_functions_agree_with_the_kernels(name):
+    call, where, args = inputs()[name]
+    assert shapes(flat(call(*[t.clone() for t in args]))) == shapes(flat(inputs('meta')[name][0](*[t.to('meta') for t in args])))
+    if where:
+        run, args = with_gradient(name)
+        meta, margs = with_gradient(name, 'meta')
+        assert shapes(run(*args)) == shapes(meta(*margs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', NAMES)
+def test_torchs_own_checks_of_an_operator(name):
+    _, where, args = inputs()[name]
+    M = ops()
+    full = {'linear_attention': lambda: (*args[:4], None, args[4], 0.5), 'linear_attention_step': lambda: (*args[:4], args[4], None, 0.5),
+            'group_norm_act': lambda: (args[0], 4, *args[1:], 1e-5, 'SiLU'), 'linear_act': lambda: (*args, 'Tanh')}[name]()
+    full = tuple(t.clone().requires_grad_(True) if any(t is args[i] for i in where) else t for t in full)
+    torch.library.opcheck(getattr(M, name).default, full, test_utils=('test_schema', 'test_autograd_registration', 'test_faketensor'))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', HALVES)
+def test_a_compiled_call_gives_the_same(name):
+    """Ahead-of-time traced, forward and backward, and run as the trace stands."""
+    call, where, args = inputs()[name]
+    compiled = torch.compile(lambda *a: flat(call(*a)), backend='aot_eager', fullgraph=True)
+
+    def run(fn):
+        leaves = [t.clone().requires_grad_(True) if i in where else t for i, t in enumerate(args)]
+        out = flat(fn(*leaves))
+        return [t.detach() for t in out] + list(torch.autograd.grad(out, [leaves[i] for i in where], [torch.ones_like(t) for t in out]))
+    assert all(torch.equal(a, b) for a, b in zip(run(compiled), run(call)))
