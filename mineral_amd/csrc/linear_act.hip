@@ -206,42 +206,39 @@ template <typename T, int N> __device__ __forceinline__ void store_row(T* p, int
   }
 }
 
-// An activation's slope (magnitude below 2) in 16 bits: sign, EXP bits of exponent, the others mantissa, rounded to nearest.  What the
-// backward pass needs of z, in z's room: rounded z, or slopes in the type itself, would add as much error to the gradients as their
-// own rounding.  Beside bf16 EXP = 4: off by 2^-12 of the slope (2^-26 below 2^-14); beside fp16 EXP = 3: 2^-13 (2^-20 below 2^-6).
-// All ones stand for NaN.
-template <int EXP> struct Slope16 {
-  static constexpr int SHIFT = 8 + EXP;                                  // bits of an fp32 mantissa that go
-  static constexpr float DOWN = EXP == 4 ? 0x1p-112f : 0x1p-120f, BACK = EXP == 4 ? 0x1p112f : 0x1p120f;
+// An activation's slope (magnitude below 1.25) in 16 bits beside 16-bit types: its sign and the fourth root of its magnitude in 15 bits,
+// steps of 1/30720.  What the backward pass needs of z, in z's room: rounded z, or slopes in the type itself, would add as much error to
+// the gradients as their own rounding.  Steps of a root get finer with the slope, so that saturated units keep theirs: off by 2^-13.9
+// of a slope of 1, 2^-12.9 at 2^-4, 2^-10.4 at 2^-14, 2^-9.9 at 2^-16 (fp16 itself: 2^-11 down to 2^-14, 2^-9 at 2^-16), and zero only
+// below 2^-63.  Zero and one are exact, the two square roots and the decoding add 2^-20.  All ones stand for NaN.
+struct Slope16 {
+  static constexpr float STEPS = 30720.0f, BACK = 1.0f / (STEPS * STEPS * STEPS * STEPS);
   static __device__ __forceinline__ unsigned pack(float s) {
-    const unsigned sign = (__float_as_uint(s) >> 16) & 0x8000u;
-    unsigned a = __float_as_uint(__builtin_fabsf(s) * DOWN);            // now the exponent fits (subnormals included)
-    a = (a + (1u << (SHIFT - 1)) - 1u + ((a >> SHIFT) & 1u)) >> SHIFT;
-    return (__builtin_fabsf(s) < 1.9f ? a : 0x7fffu) | sign;
+    const float a = __builtin_fabsf(s), q = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(a));
+    const unsigned u = (unsigned)(int)__builtin_fmaf(q, STEPS, 0.5f);
+    return (a < 1.25f ? u : 0x7fffu) | ((__float_as_uint(s) >> 16) & 0x8000u);
   }
   static __device__ __forceinline__ float unpack(unsigned u) {
-    const float a = __uint_as_float((u & 0x7fffu) << SHIFT) * BACK;
+    const float q = (float)(int)(u & 0x7fffu), q2 = q * q, a = q2 * q2 * BACK;
     return (u & 0x7fffu) == 0x7fffu ? __builtin_nanf("") : (u & 0x8000u) ? -a : a;
   }
 };
-template <typename T> struct SlopeCode { typedef Slope16<4> C; };
-template <> struct SlopeCode<_Float16> { typedef Slope16<3> C; };
 template <typename T> struct SlopeOf { typedef unsigned short S; };
 template <> struct SlopeOf<float> { typedef float S; };
-template <typename T, typename S> __device__ __forceinline__ void load_slopes(const S* p, int left, float (&x)[8]) {
+template <typename S> __device__ __forceinline__ void load_slopes(const S* p, int left, float (&x)[8]) {
   if constexpr (sizeof(S) == 4) load_row<float, 8>(p, left, x);
   else {
     const u32x4 w = load_unit<__bf16>(reinterpret_cast<const __bf16*>(p), left);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = SlopeCode<T>::C::unpack((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+    for (int e = 0; e < 8; ++e) x[e] = Slope16::unpack((w[e / 2] >> (16 * (e & 1))) & 0xffffu);
   }
 }
-template <typename T, typename S> __device__ __forceinline__ void store_slopes(S* p, int left, const float (&x)[8]) {
+template <typename S> __device__ __forceinline__ void store_slopes(S* p, int left, const float (&x)[8]) {
   if constexpr (sizeof(S) == 4) store_row<float, 8>(p, left, x);
   else {
     u32x4 w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = SlopeCode<T>::C::pack(x[2 * e]) | SlopeCode<T>::C::pack(x[2 * e + 1]) << 16;
+    for (int e = 0; e < 4; ++e) w[e] = Slope16::pack(x[2 * e]) | Slope16::pack(x[2 * e + 1]) << 16;
     typedef u32x4 __attribute__((aligned(2))) unit;
     if (left >= 8) __builtin_nontemporal_store(w, reinterpret_cast<unit*>(p));
     else {
@@ -293,7 +290,7 @@ template <typename T, int ACT, bool RES> __device__ __forceinline__ void finish8
     typedef typename SlopeOf<T>::S S;
     float d[8];
     act_slope<8>(ACT, v, d);
-    store_slopes<T>(static_cast<S*>(p.slope) + at, left, d);
+    store_slopes(static_cast<S*>(p.slope) + at, left, d);
   }
   act_fwd<8>(ACT, v);
   if constexpr (RES) {
@@ -549,7 +546,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* _
       for (int u = 0; u < U; ++u)
         if (m + 8 * u < m1) {
           load_row<T, 8>(dy + (m + 8 * u) * N + c, left, d[u]);
-          if (slope) load_slopes<T>(slope + (m + 8 * u) * N + c, left, g[u]);
+          if (slope) load_slopes(slope + (m + 8 * u) * N + c, left, g[u]);
         }
 #pragma unroll
       for (int u = 0; u < U; ++u)
