@@ -528,9 +528,10 @@ __global__ __launch_bounds__(WM * WN * WK * 64, DIRECT && NST == 3 ? 3 : 2) void
 // dz = dy slope, rounded to T as an operand of the two products (with the results' own rounding that makes 1.4 times the error of one;
 // a second term would double both products: 180 us of 400 at 32768 x 512 -> 2048), and the sums of its columns, unrounded, over this block's
 // rows -> part [blocks in y][N], or db where one block has all rows (a launch less for small batches).  32 units of 8 columns x 8 rows a block.
+// cuts: a slope of zero drops dy, whatever it is (the rectifier, as in torch); beside the other activations a dy that is not finite stays so.
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* __restrict__ slope, const T* __restrict__ dy, T* __restrict__ dz, float* __restrict__ part,
-                                                 T* __restrict__ db, int64_t M, int N, int rows) {
+                                                 T* __restrict__ db, int64_t M, int N, int rows, bool cuts) {
   __shared__ float red[8][32 * 8 + 1];
   const int cu = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + cu) * 8, left = N - c;
@@ -553,7 +554,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* _
         if (m + 8 * u < m1) {
           if (slope) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[u][e] = g[u][e] == 0.0f ? 0.0f : d[u][e] * g[u][e];
+            for (int e = 0; e < 8; ++e) d[u][e] = cuts && g[u][e] == 0.0f ? 0.0f : d[u][e] * g[u][e];
             store_row<T, 8>(dz + (m + 8 * u) * N + c, left, d[u]);
           }
 #pragma unroll
@@ -738,7 +739,7 @@ int backward(const mrl_linear* p, const void* x, const void* w, const void* slop
   if (p->rows > 0 && (db || (act && (dx || dw))))
     hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)cdiv(p->outputs, 256), r.parts), dim3(256), 0, st,
                        act ? static_cast<const typename SlopeOf<T>::S*>(slope) : nullptr, static_cast<const T*>(dy), dz, db && !whole ? part : nullptr,
-                       whole ? static_cast<T*>(db) : nullptr, p->rows, p->outputs, r.rows);
+                       whole ? static_cast<T*>(db) : nullptr, p->rows, p->outputs, r.rows, p->act == MRL_ACT_RELU);
   if (db && !whole) hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)cdiv(p->outputs, 32)), dim3(1024), 0, st, part, p->rows > 0 ? r.parts : 0, p->outputs, static_cast<T*>(db));
   const void* d = act ? static_cast<const void*>(dz) : dy;
   if (dx && p->rows > 0 && p->inputs > 0) {

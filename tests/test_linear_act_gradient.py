@@ -1,5 +1,5 @@
-"""What the gradient of torch.ops.mineral.linear_act has to survive: units in the tails of their activation, and
-offsets beyond 32 bits.
+"""What the gradient of torch.ops.mineral.linear_act has to survive: units in the tails of their activation, values that are not
+finite, and offsets beyond 32 bits.
 
 Tolerances.  u = 2^-24.  A slope is evaluated in fp32, off by (4|z| + 16) u of itself (tanh, exponential: the rounded argument of an
 exponential of up to 2|z|, and a dozen operations), for SiLU and GELU of the magnitudes of their two terms (GELU's arguments are
@@ -84,6 +84,37 @@ def test_slopes_of_zero_and_one_are_exact(dtype):
         _, dw, db = torch.autograd.grad(ops().linear_act(*leaves, None, act), leaves, dy.to(DEV))
         at = torch.ones_like(z, dtype=torch.bool) if act == 'ReLU' else z > 0
         assert torch.equal(db.cpu()[at], (want * dy[0])[at]) and torch.equal(dw[:, 0].cpu()[at], (want * dy[0])[at])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+@pytest.mark.parametrize('act,z', [('SiLU', -300.0), ('ELU', -300.0), ('Tanh', 60.0), ('GELU', -40.0), ('SiLU', 1.0), ('ReLU', 2.0)])
+def test_a_gradient_that_is_not_finite_stays_so(dtype, bad, act, z):
+    """Also where the unit is saturated: zero times NaN or infinity is no number, as in torch."""
+    dt = DT[dtype]
+    dy = torch.ones(3, 2, dtype=dt)
+    dy[1, 1] = bad
+    x, w, b = torch.ones(3, 1, dtype=dt), torch.tensor([[1.0], [z]], dtype=dt), torch.zeros(2, dtype=dt)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops().linear_act(*leaves, None, act), leaves, dy.to(DEV))
+    assert torch.isfinite(dx).cpu().flatten().tolist() == [True, False, True]
+    assert torch.isfinite(dw).cpu().flatten().tolist() == [True, False] and torch.isfinite(db).cpu().tolist() == [True, False]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_the_rectifier_drops_what_it_cut(dtype, bad):
+    """As in torch: no gradient passes a rectifier below zero, whatever it is."""
+    dt = DT[dtype]
+    dy = torch.ones(3, 2, dtype=dt)
+    dy[1, 1] = bad
+    x, w, b = torch.ones(3, 1, dtype=dt), torch.tensor([[1.0], [-2.0]], dtype=dt), torch.zeros(2, dtype=dt)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops().linear_act(*leaves, None, 'ReLU'), leaves, dy.to(DEV))
+    assert torch.equal(dx.cpu(), torch.ones(3, 1, dtype=dt))
+    assert dw.cpu().flatten().tolist() == [3.0, 0.0] and db.cpu().tolist() == [3.0, 0.0]
 
 
 @pytest.mark.gpu
