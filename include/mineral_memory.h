@@ -101,8 +101,9 @@ int mrl_linear_act(const mrl_linear* p, const void* x, const void* weight, const
 int64_t mrl_linear_act_backward_workspace_bytes(const mrl_linear* p);
 
 /* dx [rows][inputs], d_weight [outputs][inputs], d_bias [outputs], contiguous; a NULL output is not computed.  The residual's gradient
- * is dy itself.  dz = dy slope is rounded to dtype before the products; d_bias sums it unrounded.  Where MRL_ACT_RELU
- * cuts, dy is dropped, whatever it is; beside the other activations a dy that is not finite makes a dz that is not, saturated or not. */
+ * is dy itself.  dz = dy slope is rounded to dtype before the products (beside fp16 with room for every finite dy); d_bias sums it
+ * unrounded.  Where MRL_ACT_RELU cuts, dy is dropped, whatever it is; beside the other activations a dy that is not finite makes a dz
+ * that is not, saturated or not. */
 int mrl_linear_act_backward(const mrl_linear* p, const void* x, const void* weight, const void* slope, const void* dy, void* dx, void* d_weight, void* d_bias,
                             void* workspace, int64_t workspace_bytes, void* stream);
 

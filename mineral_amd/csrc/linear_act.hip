@@ -13,6 +13,8 @@
 // of this shape by the library run at 759.  8192^3: dW 1.07 PFLOP/s.  fp32, 512 -> 256, ELU: 53 us, 6 x 161 TFLOP/s of bf16 products.
 #include "memory_common.hip.h"
 
+#include <type_traits>
+
 using namespace mrl::mem;
 
 namespace {
@@ -33,6 +35,7 @@ struct MmP {
   const void *bias, *residual;
   void* slope;              // act'(z): fp32, or packed to 16 bits beside 16-bit types
   int act;
+  float gain;               // of a gradient's products beside fp16 (a power of two)
 };
 
 // one 16-byte unit, elements beyond `left` zero; addresses need only the element's alignment
@@ -365,6 +368,10 @@ template <typename T, int TM, int TN, bool PLAIN, bool RES> struct WaveEpilogue 
         }
         if (row < p.M && left > 0) {
           const int64_t at = row * p.N + c;
+          if constexpr (PLAIN && std::is_same_v<T, _Float16>) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= p.gain;
+          }
           if (PLAIN && p.slab) store_row<float, 8>(p.slab + (int64_t)t.split * p.M * p.N + at, left, v);
           else if (PLAIN) store_row<T, 8>(static_cast<T*>(p.y) + at, left, v);
           else finish8<T, ACT, RES>(p, at, left, v, bias, res[i % AHEAD][k]);
@@ -528,10 +535,12 @@ __global__ __launch_bounds__(WM * WN * WK * 64, DIRECT && NST == 3 ? 3 : 2) void
 // dz = dy slope, rounded to T as an operand of the two products (with the results' own rounding that makes 1.4 times the error of one;
 // a second term would double both products: 180 us of 400 at 32768 x 512 -> 2048), and the sums of its columns, unrounded, over this block's
 // rows -> part [blocks in y][N], or db where one block has all rows (a launch less for small batches).  32 units of 8 columns x 8 rows a block.
+// fp16 beside SiLU and GELU, whose slopes pass one, keeps shrink dz = dz / 2, which has room for every finite dy, and the products are doubled
+// (exactly, in fp32): dz itself would be infinite from dy = 58000 on.  Subnormal values of dz lose one more bit by it.
 // cuts: a slope of zero drops dy, whatever it is (the rectifier, as in torch); beside the other activations a dy that is not finite stays so.
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* __restrict__ slope, const T* __restrict__ dy, T* __restrict__ dz, float* __restrict__ part,
-                                                 T* __restrict__ db, int64_t M, int N, int rows, bool cuts) {
+                                                 T* __restrict__ db, int64_t M, int N, int rows, bool cuts, float shrink) {
   __shared__ float red[8][32 * 8 + 1];
   const int cu = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + cu) * 8, left = N - c;
@@ -555,7 +564,12 @@ __global__ __launch_bounds__(256) void dz_kernel(const typename SlopeOf<T>::S* _
           if (slope) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[u][e] = cuts && g[u][e] == 0.0f ? 0.0f : d[u][e] * g[u][e];
-            store_row<T, 8>(dz + (m + 8 * u) * N + c, left, d[u]);
+            if constexpr (std::is_same_v<T, _Float16>) {
+              float half[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) half[e] = d[u][e] * shrink;
+              store_row<T, 8>(dz + (m + 8 * u) * N + c, left, half);
+            } else store_row<T, 8>(dz + (m + 8 * u) * N + c, left, d[u]);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) s[e] += d[u][e];
@@ -736,20 +750,21 @@ int backward(const mrl_linear* p, const void* x, const void* w, const void* slop
   float* part = reinterpret_cast<float*>(ws + r.dz);
   float* slab = reinterpret_cast<float*>(ws + r.dz + r.part);
   const bool act = p->act != MRL_ACT_NONE, whole = p->rows > 0 && r.parts == 1;
+  const bool halves = p->dtype == MRL_F16 && (p->act == MRL_ACT_SILU || p->act == MRL_ACT_GELU);
   if (p->rows > 0 && (db || (act && (dx || dw))))
     hipLaunchKernelGGL((dz_kernel<T>), dim3((unsigned)cdiv(p->outputs, 256), r.parts), dim3(256), 0, st,
                        act ? static_cast<const typename SlopeOf<T>::S*>(slope) : nullptr, static_cast<const T*>(dy), dz, db && !whole ? part : nullptr,
-                       whole ? static_cast<T*>(db) : nullptr, p->rows, p->outputs, r.rows, p->act == MRL_ACT_RELU);
+                       whole ? static_cast<T*>(db) : nullptr, p->rows, p->outputs, r.rows, p->act == MRL_ACT_RELU, halves ? 0.5f : 1.0f);
   if (db && !whole) hipLaunchKernelGGL((column_sum_kernel<T>), dim3((unsigned)cdiv(p->outputs, 32)), dim3(1024), 0, st, part, p->rows > 0 ? r.parts : 0, p->outputs, static_cast<T*>(db));
   const void* d = act ? static_cast<const void*>(dz) : dy;
   if (dx && p->rows > 0 && p->inputs > 0) {
     MmP a{};
-    a.a = d; a.lda = p->outputs; a.b = w; a.ldb = p->inputs; a.M = (int)p->rows; a.N = p->inputs; a.R = p->outputs; a.r_split = p->outputs; a.y = dx;
+    a.gain = halves ? 2.0f : 1.0f; a.a = d; a.lda = p->outputs; a.b = w; a.ldb = p->inputs; a.M = (int)p->rows; a.N = p->inputs; a.R = p->outputs; a.r_split = p->outputs; a.y = dx;
     multiply<T, LAY_K, LAY_R>(a, r.edge_x, 1, st);
   }
   if (dw && p->inputs > 0) {
     MmP a{};
-    a.a = d; a.lda = p->outputs; a.b = x; a.ldb = p->x_stride; a.M = p->outputs; a.N = p->inputs; a.R = p->rows; a.r_split = r.r_split;
+    a.gain = halves ? 2.0f : 1.0f; a.a = d; a.lda = p->outputs; a.b = x; a.ldb = p->x_stride; a.M = p->outputs; a.N = p->inputs; a.R = p->rows; a.r_split = r.r_split;
     if (r.splits > 1) a.slab = slab;
     else a.y = dw;
     multiply<T, LAY_R, LAY_R>(a, r.edge_w, r.splits, st);

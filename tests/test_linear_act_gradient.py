@@ -1,5 +1,5 @@
 """What the gradient of torch.ops.mineral.linear_act has to survive: units in the tails of their activation, values that are not
-finite, and offsets beyond 32 bits.
+finite, fp16 gradients near the type's largest value, and offsets beyond 32 bits.
 
 Tolerances.  u = 2^-24.  A slope is evaluated in fp32, off by (4|z| + 16) u of itself (tanh, exponential: the rounded argument of an
 exponential of up to 2|z|, and a dozen operations), for SiLU and GELU of the magnitudes of their two terms (GELU's arguments are
@@ -115,6 +115,38 @@ def test_the_rectifier_drops_what_it_cut(dtype, bad):
     dx, dw, db = torch.autograd.grad(ops().linear_act(*leaves, None, 'ReLU'), leaves, dy.to(DEV))
     assert torch.equal(dx.cpu(), torch.ones(3, 1, dtype=dt))
     assert dw.cpu().flatten().tolist() == [3.0, 0.0] and db.cpu().tolist() == [3.0, 0.0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ['SiLU', 'GELU'])
+@pytest.mark.parametrize('shape', [(1, 1, 1), (5, 40, 33), (70, 96, 128), (2100, 72, 264), (5000, 130, 520), (9000, 264, 1000), (1100, 1048, 1032), (16400, 200, 1024)])
+def test_fp16_gradients_near_the_largest_value(act, shape):
+    """Slopes of SiLU and GELU reach 1.13: dy slope passes 65504 where dy does not, while its products with small weights and inputs are
+    ordinary numbers."""
+    M, K, N = shape
+    dt = torch.float16
+    g = torch.Generator().manual_seed(21)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g).double() * 2 - 1  # noqa: E731
+    # powers of two, so that z = 1.5 + x w is nearly 1.5 (slope over 1.04) and the results stay below 65504
+    x = (2.0 ** -11 * (1 + torch.rand(M, K, generator=g).double()) * sign(M, K)).to(dt)
+    w = (2.0 ** -11 * (1 + torch.rand(N, K, generator=g).double()) * sign(N, K)).to(dt)
+    b, dy = torch.full((N,), 1.5).to(dt), (sign(M, N) * 65504).to(dt)
+    print(f'large fp16 gradients {shape} {act}', flush=True)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    dx, dw, _ = torch.autograd.grad(ops().linear_act(*leaves, None, act), leaves, dy.to(DEV))
+    x, w, b, dy = (t.double() for t in (x, w, b, dy))
+    z = x @ w.t() + b
+    s, e = slope_error(z, act, dt)
+    e = e + 1.13 * (K + 16) * U * (x.abs() @ w.abs().t() + b)
+    dz = dy * s
+    assert float(dz.abs().max()) > 65504 * 1.03
+    dze = dy.abs() * e + la.half_of(dt) * (dy.abs() * (s.abs() + e))
+    for n, a, ref, lim in (('dx', dx, dz @ w, dze @ w.abs() + (N + 16) * U * ((dz.abs() + dze) @ w.abs())),
+                           ('d_weight', dw, dz.t() @ x, dze.t() @ x.abs() + (M + 16) * U * ((dz.abs() + dze).t() @ x.abs()))):
+        assert float(ref.abs().max()) < 65504
+        err = (a.double().cpu() - ref).abs()
+        lim = lim + la.half_of(dt) * (ref.abs() + lim) + half_spacing(dt)
+        assert bool((err <= lim).all()), f'{n}: worst {float((err / lim).max()):.2f} of the bound'
 
 
 @pytest.mark.gpu
