@@ -11,8 +11,9 @@
 //     launch leaves count, mean and sum of squares of its part, the second joins the parts and writes y; backwards the first
 //     leaves the two sums of each channel, a small one joins them, the third writes dx.  The second reading of x comes from the
 //     256 MB cache behind the L2s where the data fit it.
-// Means and variances are joined pairwise (count, mean, centred squares), so a large mean costs no digits.  Every sum has one
-// order: no atomics.
+// Means and variances are joined pairwise (count, mean, centred squares), so a large mean costs no digits.  The mean of equal values is
+// their value, so that such a group has no spread (a spacing of the mean, divided by sqrt(eps), would show): of 16-bit values by exact
+// sums and true quotients, of fp32 ones by taking off the mean of what the first mean leaves.  Every sum has one order: no atomics.
 #include "memory_common.hip.h"
 
 #include <type_traits>
@@ -110,6 +111,12 @@ template <int TL> __device__ __forceinline__ float team_sum(float v) {
   return v;
 }
 
+// A product as it is rounded: not to be fused into the difference that follows, which would be taken of another mean than is kept.
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 // ---- one pixel per sample --------------------------------------------------------------------------------------------------------
 // Row r = n G + g is Cg contiguous values.  A team of TL lanes, NV vectors per lane, walks the rows team, team + teams, ... of its group.
 // RAG: Cg is not a number of whole vectors, and rows lie on any address.
@@ -153,15 +160,39 @@ __global__ __launch_bounds__(256) void token_fwd_kernel(const GnP p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) s += v[i][e];
       }
-    const float mean = team_sum<TL>(s) * inv;
+    // The sum of up to 2048 equal values of 16 bits is exact and its quotient their value; an fp32 mean is freed of its rounding by the
+    // mean of what it leaves.
+    float mean = sizeof(T) == 2 ? team_sum<TL>(s) / (float)p.Cg : rounded(team_sum<TL>(s) * inv);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (in[i]) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          v[i][e] -= mean;
-          if (!RAG || e < left(i)) q = __builtin_fmaf(v[i][e], v[i][e], q);
+        for (int e = 0; e < V; ++e) v[i][e] -= mean;
+      }
+    if constexpr (sizeof(T) == 4) {
+      float d = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (in[i]) {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (!RAG || e < left(i)) d += v[i][e];
         }
+      d = team_sum<TL>(d) * inv;
+      mean += d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (in[i]) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[i][e] -= d;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (in[i]) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (!RAG || e < left(i)) q = __builtin_fmaf(v[i][e], v[i][e], q);
       }
     const float rstd = 1.0f / sqrtf(team_sum<TL>(q) * inv + p.eps);
 #pragma unroll
@@ -389,14 +420,23 @@ __global__ __launch_bounds__(256) void pixel_stats_kernel(const GnP p) {
 #pragma unroll
           for (int e = 0; e < V; ++e) a += v[u][e];
         }
-      const float mb = a / k;
-      float sb = 0.0f;
+      float mb = a / k, sb = 0.0f, d = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (r + (int64_t)u * q.rows < q.p1) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) sb = __builtin_fmaf(v[u][e] - mb, v[u][e] - mb, sb);
+          for (int e = 0; e < V; ++e) {
+            const float c = v[u][e] - mb;
+            if constexpr (sizeof(T) == 4) d += c;
+            sb = __builtin_fmaf(c, c, sb);
+          }
         }
+      if constexpr (sizeof(T) == 4) {
+        d /= k;
+        mb += d;
+        sb = __builtin_fmaf(-d * k, d, sb);
+        sb = sb < 0.0f ? 0.0f : sb;
+      }
       join_moments(n, m, s, k, mb, sb);
     }
   }
@@ -450,14 +490,25 @@ __global__ __launch_bounds__(256) void pixel_stats_mixed_kernel(const GnP p) {
       const float ik = 1.0f / k, t = n + k, f = k / t, g = n * f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        float a = 0.0f, b = 0.0f;
+        float a = 0.0f, b = 0.0f, o = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (r + (int64_t)u * q.rows < q.p1) a += v[u][e];
-        a *= ik;
+        if (sizeof(T) == 4 || k == (float)U) a = rounded(a * ik);
+        else a /= k;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (r + (int64_t)u * q.rows < q.p1) b = __builtin_fmaf(v[u][e] - a, v[u][e] - a, b);
+          if (r + (int64_t)u * q.rows < q.p1) {
+            const float x = v[u][e] - a;
+            if constexpr (sizeof(T) == 4) o += x;
+            b = __builtin_fmaf(x, x, b);
+          }
+        if constexpr (sizeof(T) == 4) {
+          const float h = o * ik;
+          a += h;
+          b = __builtin_fmaf(-h, o, b);
+          b = b < 0.0f ? 0.0f : b;
+        }
         const float d = a - m[e];
         m[e] = __builtin_fmaf(d, f, m[e]);
         s[e] += b + d * d * g;
