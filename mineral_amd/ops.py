@@ -9,11 +9,13 @@ calling an operator with CPU tensors fails in the dispatcher instead of falling 
     torch.ops.mineral.gae_finish(rewards_tn, values_tn, dones_tn, neglogp_tn, last_values, 0.99, 0.95, ...)
 
 The operators of a sequence memory (linear_attention, linear_attention_step, group_norm_act, linear_act) are differentiable and
-registered by memory_ops, which this module imports.
+registered by memory_ops, which this module imports; where their library is missing it says so in a warning and goes on without them.
 
 Network description for the operators that run the towers: `net_i` = [obs_dim, act_dim, dist_type, tower_kind, fixed_sigma,
 units...] (dist_type 0 normal / 1 dreamerv3_normal; tower_kind 0 LayerNorm+SiLU / 1 ELU / 2 LayerNorm+ELU) and `net_f` = [minstd, maxstd, ln_eps].
 """
+
+import warnings
 
 import torch
 
@@ -143,6 +145,11 @@ for _name, _fn in (('rollout_write', _rollout_write), ('gae_finish', _gae_finish
 
 OPS = ('workspace_bytes', 'param_count', 'rollout_write', 'gae_finish', 'welford_update_', 'normalize_clamp', 'policy_act', 'ppo_grad', 'clip_adam_step_')
 
-from . import memory_ops as _memory_ops  # noqa: E402  (linear attention, group norm, linear layer: include/mineral_memory.h)
-
-OPS += _memory_ops.OPS
+# linear attention, group norm, linear layer (include/mineral_memory.h): host code of their own, built against one version of torch.  Without
+# it they are not there, and what is registered above serves all the same.
+try:
+    from . import memory_ops as _memory_ops  # noqa: E402
+except (_hip.HipLibraryError, OSError) as _error:
+    warnings.warn(f'torch.ops.mineral has no memory operators (linear_attention, group_norm_act, linear_act): {_error}')
+else:
+    OPS += _memory_ops.OPS
