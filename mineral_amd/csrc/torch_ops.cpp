@@ -17,6 +17,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -275,6 +276,7 @@ Tensor linear_attention_step_autograd(c10::DispatchKeySet ks, const Tensor& q, c
 // Reached in inference mode too, where autograd is not: what a step overwrites is marked as written.
 Tensor linear_attention_step_inplace(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& l, const Tensor& state, const OptT& r, double scale) {
   static const auto fwd = op<StepSig>("mineral::linear_attention_step");
+  TORCH_CHECK(!state.is_inference() || c10::InferenceMode::is_enabled(), "linear_attention_step: a state made in inference mode is updated there only");
   Tensor out;
   {
     const at::AutoDispatchBelowADInplaceOrView below;

@@ -283,3 +283,45 @@ def test_a_compiled_call_gives_the_same(name):
         out = flat(fn(*leaves))
         return [t.detach() for t in out] + list(torch.autograd.grad(out, [leaves[i] for i in where], [torch.ones_like(t) for t in out]))
     assert all(torch.equal(a, b) for a, b in zip(run(compiled), run(call)))
+
+
+@pytest.mark.gpu
+def test_a_compiled_step_updates_its_state():
+    call, _, args = inputs()['linear_attention_step']
+    compiled = torch.compile(lambda *a: call(*a), backend='aot_eager', fullgraph=True)
+    mine, theirs = args[4].clone(), args[4].clone()
+    with torch.no_grad():
+        for _ in range(3):
+            assert torch.equal(compiled(*args[:4], mine), call(*args[:4], theirs)) and torch.equal(mine, theirs)
+
+
+@pytest.mark.gpu
+def test_states_of_inference_mode():
+    """Updated there, and outside refused before anything is written."""
+    call, _, args = inputs()['linear_attention_step']
+    want = args[4].clone()
+    out = call(*args[:4], want)
+    with torch.inference_mode():
+        state = args[4].clone()
+        assert torch.equal(call(*args[:4], state), out) and torch.equal(state, want)
+        held = state.clone()
+    with pytest.raises(RuntimeError, match='inference'):
+        call(*args[:4], state)
+    assert torch.equal(state, held)
+    q, k, v, l = (t.clone() for t in args[:4])
+    with torch.inference_mode():
+        others = [t.clone() for t in (q, k, v, l)]
+    with pytest.raises(RuntimeError, match='inference'):
+        call(*others, state)
+    assert torch.equal(state, held)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', HALVES)
+def test_a_call_mapped_over_a_batch(name):
+    """torch.vmap has no rule for the operators and calls them one by one."""
+    call, where, args = inputs()[name]
+    x = torch.stack([args[0], args[0] * 0.5, -args[0]])
+    got = flat(torch.vmap(lambda t: call(t, *args[1:]))(x))
+    want = [torch.stack(ts) for ts in zip(*(flat(call(t, *args[1:])) for t in x))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
