@@ -26,8 +26,8 @@ extern "C" {
  *     o_t = scale * S_t^T q_t
  * for every batch row b and head h, with S of dim_k x dim_v in fp32.  A reset drops whatever the state held, NaN and infinity
  * included, and no token's output depends on a later token or on an earlier episode.  log_decay <= 0 is meant; -inf keeps nothing of a
- * finite state.  fp32 products are formed from three bf16 terms, exact from magnitudes of 2^-100 on (an infinite value makes NaN of what
- * it belongs to); the state and all sums are fp32.  batch x heads is below 2^23.
+ * finite state.  fp32 products are formed from three bf16 terms, exact for magnitudes from 2^-100 to 3.38e38 (a larger or infinite value
+ * makes NaN of what it belongs to); the state and all sums are fp32.  batch x heads is below 2^23.
  *   q, k : [batch][steps][heads][dim_k], v : [batch][steps][heads][dim_v] of `dtype`; strides {batch, step, head}
  *   log_decay : [heads] fp32;  resets : [batch][steps] bytes or NULL;  initial_state : [batch][heads][dim_k][dim_v] fp32 or NULL (zero) */
 typedef struct mrl_attention {
@@ -88,7 +88,8 @@ int mrl_group_norm_act_backward(const mrl_group_norm* p, const void* x, const vo
 /* Linear layer: y = act(x W^T + bias) + residual.
  *   x : [rows][inputs], row stride x_stride; weight : [outputs][inputs]; bias : [outputs] or NULL; residual : [rows][outputs] or NULL;
  *   y : [rows][outputs]; all of `dtype`, contiguous but for x.  16-bit operands multiply as they are and fp32 ones as three exact
- *   bf16 terms (six products, error below an fp32 product's rounding, for magnitudes from 2^-100 on; an infinite operand gives NaN); everything accumulates in fp32 and is rounded once. */
+ *   bf16 terms (six products, error below an fp32 product's rounding, for magnitudes from 2^-100 to
+ *   3.38e38; a larger or infinite operand gives NaN); everything accumulates in fp32 and is rounded once. */
 typedef struct mrl_linear {
   int64_t rows, x_stride;
   int32_t inputs, outputs, dtype, act;

@@ -10,7 +10,8 @@
 //   * many pixels: blocks take runs of pixels with all (up to 256 vectors of) channels, a thread always the same ones.  The first
 //     launch leaves count, mean and sum of squares of its part, the second joins the parts and writes y; backwards the first
 //     leaves the two sums of each channel, a small one joins them, the third writes dx.  The second reading of x comes from the
-//     256 MB cache behind the L2s where the data fit it.
+//     256 MB cache behind the L2s where the data fit it.  Tokens whose group no team holds (over 256 vectors) come here too, one pixel
+//     each: two readings, and backwards a workspace of 16 bytes a value (65536 x 4096 in one group, bf16: 1.0 ms forward, 3.8 backward).
 // Means and variances are joined pairwise (count, mean, centred squares), so a large mean costs no digits.  The mean of equal values is
 // their value, so that such a group has no spread (a spacing of the mean, divided by sqrt(eps), would show): of 16-bit values by exact
 // sums and true quotients, of fp32 ones by taking off the mean of what the first mean leaves.  Every sum has one order: no atomics.

@@ -9,7 +9,7 @@
 // fp32 operands are split exactly into three bf16 terms on their way to LDS and multiply in six products, smallest first.
 // dW sums over all rows: they are split over blocks whose partial sums are added in a fixed order.
 // Bound: 32768 rows, 512 -> 2048, bf16, SiLU, residual: forward 165 us (435 MB to move and 69 GFLOP; the epilogue's loads and stores
-// beside products of 16 steps only), dz 86 us (403 MB, 4.7 TB/s), dx 83 us (828 TFLOP/s), dW 95 + 7 us (723 TFLOP/s); plain products
+// beside products of 16 steps only), dz 88 us (403 MB, 4.6 TB/s), dx 84 us (818 TFLOP/s), dW 95 + 7 us (723 TFLOP/s); plain products
 // of this shape by the library run at 759.  8192^3: dW 1.07 PFLOP/s.  fp32, 512 -> 256, ELU: 53 us, 6 x 161 TFLOP/s of bf16 products.
 #include "memory_common.hip.h"
 

@@ -24,9 +24,11 @@
 // the rate of the fp32 MFMA.
 //
 // Bound: by memory where there are many sequences (8192 of 32 tokens, 64 x 64, fp32, states in and out: 111 us for 0.54 GB, 4.8 TB/s;
-// their gradient, three scans in six-term products, 260 us for 0.87 GB), by the latency of one chunk after the other, about 4 us
-// in fp32 and 2 in 16 bits, where few sequences are long (8 of 16384 tokens, 128 x 128, bf16: 27 us for the segments' states, 11 to
-// join them, 57 for the outputs).
+// their gradient about 275 us for 1.38 GB, 5.0 TB/s: its three scans run one after the other and read q, k, v and d_out again, 1.02 GB
+// instead of 0.54); by the latency of one chunk after the other where few sequences are long: 4.5 us for 64 tokens in 16 bits at 64 x 64
+// (272 blocks of 655 tokens: 49 us), 4.6 for 32 in fp32 (96 us), and 7 for 64 at 128 x 128, where each of eight waves computes all scores
+// for its 16 columns and one block fills a CU (8 sequences of 16384 tokens, bf16: 27 us for the segments' states, 3.4 a chunk, 12 to join
+// them, 57 for the outputs).
 //
 // Masked tokens: weights are applied by selection, and a chunk that holds an infinity or NaN is walked token by token (the same
 // code with chunks of one), so that a zero weight never meets one: nothing of a later token or an earlier episode leaks.
