@@ -127,3 +127,25 @@ def test_gradients_beside_what_a_reset_drops(dtype, T, bad_at, end, bad):
         for n, a, r, m, keep in zip(('dq', 'dk', 'dv'), got, ref, mag, clean[which]):
             check(a[:, keep.to(DEV)], r[:, keep], m[:, keep], DT[dtype], T, max(K, V), f'{n} beside a bad {which}')
         assert torch.equal(got[3], torch.zeros_like(got[3]))
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_the_31_outputs():
+    """32769 rows of equal queries and keys: the last, whose outputs and gradients lie beyond 2^31, has the bits of a call of its own."""
+    B, T, H, K = 2 ** 15 + 1, 64, 32, 32
+    q, k, v, l, r, s = at.dev(*at.make(1, T, H, K, K, torch.bfloat16, 43))
+    g = torch.Generator(device=DEV).manual_seed(44)
+    big = torch.randn(B, T, H, K, generator=g, device=DEV, dtype=torch.bfloat16)
+    do = torch.randn(B, T, H, K, generator=g, device=DEV, dtype=torch.bfloat16)
+    big[0], big[-1], do[0], do[-1] = v[0], v[0], 1, 1
+
+    def both(q, k, v, r, do):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o, f = at.ops().linear_attention(*leaves, l, r, None, 0.25)
+        return (o.detach(), f.detach(), *torch.autograd.grad(o, leaves, do))
+
+    got = both(q.expand(B, T, H, K), k.expand(B, T, H, K), big, r.expand(B, T), do)
+    want = both(q, k, v, r, torch.ones_like(v))
+    assert got[0].numel() > 2 ** 31
+    for a, b in zip(got, want):
+        assert torch.equal(a[-1], b[0]) and torch.equal(a[0], b[0])
